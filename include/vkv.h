@@ -62,7 +62,12 @@ typedef enum vkv_dtype {
     /* model weights (ggml block formats, 256 elements per block) */
     VKV_DTYPE_Q4_K = 12,   /* 144 B: fp16 d, fp16 dmin, 6-bit scales/mins, 4-bit codes */
     VKV_DTYPE_Q6_K = 14,   /* 210 B: 4+2-bit codes, int8 scales per 16, fp16 d */
-    VKV_DTYPE_Q8_K = 15    /* 292 B: f32 d, int8 codes, int16 sums per 16 (activations) */
+    VKV_DTYPE_Q8_K = 15,   /* 292 B: f32 d, int8 codes, int16 sums per 16 (activations) */
+    /* codes of paged K/V (ggml's number for int8; e4m3 has none) */
+    VKV_DTYPE_I8 = 24,
+    VKV_DTYPE_E4M3 = 100,  /* 8-bit float, 4 exponent and 3 mantissa bits, largest 448 */
+    /* rows of the batched serving operators */
+    VKV_DTYPE_BF16 = 30
 } vkv_dtype;
 
 /* Decoder ring metadata: voxtral_decoder_kv_ring (src/voxtral-internal.h:195-204).
@@ -776,6 +781,132 @@ const void *vkv_model_tensor(const vkv_model *model, const char *name, vkv_gguf_
  * dec.layers[l].ada_scale = scales + l * dim).  A model without ada
  * conditioning leaves the view alone. */
 vkv_status vkv_model_set_ada(vkv_model *model, float t, float *scales, void *hip_stream);
+
+/* ---------------------------------------------------------------------------
+ * Many requests over one pool of 8-bit K/V pages.
+ *
+ * A pool holds n_pages pages of page_size tokens for every layer; a request
+ * owns the pages of its row of a block table ([n_req][table_stride] page ids,
+ * entry i for tokens [i * page_size, (i + 1) * page_size)).  Codes are one
+ * byte, with one scale per page and kv head, a power of two: an element is
+ * code * scale[layer][page][kv_head].  K codes are
+ * [layer][page][kv_head][page_size][head_dim].  V codes are stored by blocks
+ * of 16 tokens with the token innermost: of a page and head, token 16 b + 4 g
+ * + j (j < 4) and dim 16 t + r (r < 16) is at byte
+ *   (((b * 16 + r) * 4 + g) * (head_dim / 16) + t) * 4 + j.
+ * The memory is the caller's; nothing in it needs to be set before a page's
+ * first token is appended.  Rows of q, k, v and out are VKV_DTYPE_F32, _F16 or
+ * _BF16; row strides count elements (0 = packed).  Rows are 16-byte aligned
+ * (logits: their array), int32 and f32 arrays 4-byte.  Calls run on the device of their stream (the
+ * current one for the null stream), allocate nothing and may be captured in a
+ * HIP graph.  Calls that run at the same time need workspaces of their own.
+ * ------------------------------------------------------------------------- */
+typedef struct vkv_pages {
+    void *k, *v;               /* codes: n_layers * n_pages * n_kv_heads * page_size * head_dim bytes each */
+    float *k_scale, *v_scale;  /* [n_layers][n_pages][n_kv_heads] */
+    int32_t dtype;             /* VKV_DTYPE_E4M3 or VKV_DTYPE_I8 */
+    int32_t n_layers;
+    int32_t n_pages;           /* n_pages * page_size < 2^31 */
+    int32_t page_size;         /* 16, 32, 64, 128 or 256 */
+    int32_t n_kv_heads;
+    int32_t head_dim;          /* 64 or 128 */
+} vkv_pages;
+
+/* A step's block tables and slots from the requests' lengths before
+ * (len_old) and after it (len_new), all device arrays.  A request that needs
+ * fewer pages than it held (a rollback, or 0: its end) returns entries
+ * [ceil(new / page_size), ceil(old / page_size)) to the free stack, requests
+ * and entries in rising order; then every request that needs more takes its
+ * new entries, in the same order, each the stack's top.  The stack is
+ * free_pages[0, *n_free) (room for n_pages ids); its new size goes to
+ * *n_free_out, which may be n_free itself.  Table entries behind a request's
+ * pages are neither read nor changed.
+ * The new tokens of all requests are packed one request behind the other:
+ * cu_new[n_req + 1] are their offsets, slots[t] = page * page_size + offset in
+ * the page and positions[t] the token's position; both are -1 for t in
+ * [cu_new[n_req], max_tokens).  len_out (which may be len_old or len_new)
+ * receives the requests' lengths.
+ * *status = 0; or 1 where the free pages do not suffice, 2 where a length is
+ * negative or beyond the table, the new tokens are more than max_tokens, or
+ * the stack or a returned entry is no page's: then nothing moves, len_out =
+ * len_old, every offset is 0 and every slot -1, so that the step's other calls
+ * do nothing. */
+vkv_status vkv_page_map(const int32_t *len_old, const int32_t *len_new, int32_t n_req,
+                        int32_t page_size, int32_t n_pages, int32_t *table, int32_t table_stride,
+                        int32_t *free_pages, const int32_t *n_free, int32_t *n_free_out,
+                        int32_t max_tokens, int32_t *len_out, int32_t *cu_new, int32_t *slots,
+                        int32_t *positions, int32_t *status, void *hip_stream);
+
+/* Append n_tokens K and V rows (n_kv_heads * head_dim values each) to one
+ * layer at the slots of a page map.  Per page and head the scale is the least
+ * power of two (2^-100 to 2^120) that holds the largest finite magnitude of
+ * the rows, and no less than the page's scale so far unless this call writes
+ * the page's slot 0, which begins it anew; where the scale of a page grows,
+ * its other codes are rounded to the new one.  Values go to the nearest code,
+ * ties to even; what is not finite becomes NaN in e4m3, and in int8 0 (NaN) or
+ * the largest code of its sign.  A slot outside the pool (-1: a token of
+ * another call, or padding) is skipped.  The tokens of one page must stand
+ * next to each other in the call, as vkv_page_map leaves them, in any order;
+ * of several rows for one slot the last counts. */
+vkv_status vkv_pages_append(const vkv_pages *pages, int32_t layer, const int32_t *slots,
+                            int32_t n_tokens, int32_t dtype, const void *k, const void *v,
+                            int64_t row_stride, void *hip_stream);
+
+/* Single-query attention with grouped heads over the pages of one layer: for
+ * row r, out[r][h] = sum_j softmax_j(scale * q[r][h] . K_j) V_j over the last
+ * min(lens[r], window) tokens (window 0: all) of the request whose block table
+ * is row r of table.  Several new tokens of one request are several rows with
+ * rising lengths over the same table entries (table_stride apart, or 0: one
+ * table for all rows).  A row of length <= 0 gives zeros; a length beyond
+ * max_len, or a page id outside the pool among the tokens attended to, NaN.
+ * max_len <= table_stride * page_size (with stride 0: the one table's pages
+ * are taken to reach max_len).  q, out: [n_rows][n_q_heads][head_dim]; the
+ * products take q and the softmax weights in 22 bits, sums are 32-bit.
+ * The workspace is 16-byte aligned; its contents do not matter. */
+size_t vkv_paged_attn_workspace(const vkv_pages *pages, int32_t n_rows, int32_t n_q_heads,
+                                int32_t max_len);
+vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *table,
+                          int32_t table_stride, const int32_t *lens, int32_t n_rows,
+                          int32_t max_len, int32_t window, int32_t dtype, const void *q,
+                          int64_t q_stride, void *out, int64_t out_stride, int32_t n_q_heads,
+                          float scale, void *workspace, size_t workspace_bytes, void *hip_stream);
+
+/* Causal attention with grouped heads over n_seq prompts packed one behind the
+ * other: rows [cu_seqlens[i], cu_seqlens[i + 1]) of q ([..][n_q_heads]
+ * [head_dim]), k and v ([..][n_kv_heads][head_dim]) and out are prompt i
+ * (device array of n_seq + 1 offsets; vkv_page_map's cu_new is one).  Token t
+ * of a prompt attends to its tokens (t - window, t] (window 0: [0, t]).  The
+ * arrays hold n_tokens rows; rows behind the last prompt are not read, and
+ * those of out are left as they are.  Prompts may be empty.  Keys that a row
+ * does not attend to have no effect on it, whatever they hold.
+ * F32 rows are multiplied as pairs of f16 (22 bits), F16 and BF16 rows as they
+ * are, with the softmax weights rounded to that type; sums are 32-bit.
+ * The workspace is 256-byte aligned; its contents do not matter. */
+size_t vkv_prompt_attn_workspace(int32_t dtype, int32_t n_seq, int32_t n_tokens,
+                                 int32_t n_kv_heads, int32_t head_dim);
+vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const void *k,
+                           int64_t k_stride, const void *v, int64_t v_stride,
+                           const int32_t *cu_seqlens, int32_t n_seq, int32_t n_tokens,
+                           int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
+                           int32_t window, void *out, int64_t out_stride, void *workspace,
+                           size_t workspace_bytes, void *hip_stream);
+
+/* Log probabilities under softmax of each row of logits ([n_rows][n_vocab]
+ * F32, F16 or BF16): of the row's given token (tokens and logprob, or both
+ * NULL), the entropy of the row in nats (or NULL), and the n_top <= 32 largest
+ * logits' ids (top_ids[n_rows][n_top], largest first, equal ones by rising id)
+ * with their log probabilities.  A logit of -inf has probability 0; in a row
+ * of nothing else every log probability is -inf and the entropy 0.  NaN or
+ * +inf in a row makes its log probabilities and entropy NaN (NaN counts as the
+ * largest).  The log probability of token -1 (a padding row) is 0, of any
+ * other id outside the vocabulary NaN.
+ * The workspace is 16-byte aligned; its contents do not matter. */
+#define VKV_LOGPROBS_MAX_TOP 32
+size_t vkv_logprobs_workspace(int32_t n_rows, int64_t n_vocab, int32_t n_top);
+vkv_status vkv_logprobs(int32_t dtype, const void *logits, int64_t row_stride, int32_t n_rows,
+                        int64_t n_vocab, const int32_t *tokens, float *logprob, float *entropy,
+                        int32_t n_top, int32_t *top_ids, float *top_logprobs, void *workspace,
+                        size_t workspace_bytes, void *hip_stream);
 
 /* ---------------------------------------------------------------------------
  * Seeded synthetic rows (integer Irwin-Hall N(0,1), bit-identical to the CPU

@@ -1,0 +1,833 @@
+// A paged 8-bit K/V cache on gfx950: the page map built from request lengths,
+// the quantizing append and the single-query attention over the pages.
+//
+// Page layout (codes, one byte each; S tokens, D dims): K is [S][D]; V is
+// stored by blocks of 16 tokens with the token innermost, token 4 g + j and
+// dim 16 t + r of a block at ((r * 4 + g) * (D / 16) + t) * 4 + j.  That is
+// the order in which the lanes of v_mfma_f32_16x16x32_f16 take the transposed
+// V: lane (r, g) reads D / 4 contiguous bytes of a block, and no byte moves
+// between lanes.
+#include <hip/hip_runtime.h>
+
+#include <cfloat>
+
+#include "vkv_serve.h"
+
+namespace vkv {
+namespace {
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// ---------------------------------------------------------------------------
+// Page map
+// ---------------------------------------------------------------------------
+
+constexpr int kMapThreads = 1024;
+
+__device__ __forceinline__ int pages_of(int len, int page) { return (int)(((int64_t)len + page - 1) / page); }
+
+struct MapReq {
+    int old_len, new_len, held, want;
+    __device__ int ret() const { return held > want ? held - want : 0; }
+    __device__ int take() const { return want > held ? want - held : 0; }
+    __device__ int grow() const { return new_len > old_len ? new_len - old_len : 0; }
+};
+
+__device__ __forceinline__ MapReq map_req(const MapArgs &a, int r) {
+    MapReq q{0, 0, 0, 0};
+    if (r < a.n_req) {
+        q.old_len = a.len_old[r];
+        q.new_len = a.len_new[r];
+        q.held = pages_of(q.old_len, a.page_size);
+        q.want = pages_of(q.new_len, a.page_size);
+    }
+    return q;
+}
+
+// inclusive sum over the work group; every thread's total in *total.  LDS:
+// one word per wave.
+__device__ __forceinline__ int block_scan(int x, int *lds, int *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kMapThreads / 64; ++w) {
+        const int s = lds[w];
+        if (w < wave) before += s;
+        all += s;
+    }
+    *total = all;
+    return x + before;
+}
+
+// first index i in [0, n) with p[i] > x (p rising), n if none
+__device__ __forceinline__ int upper_bound(const int *p, int n, int x) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (p[mid] > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+// slot and position of packed token t of request r
+__device__ __forceinline__ void map_token(const MapArgs &a, int t, int r, int pos) {
+    const int page = a.table[(int64_t)r * a.table_stride + pos / a.page_size];
+    a.slots[t] = page * a.page_size + pos % a.page_size;
+    a.positions[t] = pos;
+}
+
+// One work group: the free stack is one list, and a step's lengths are a few
+// KB.  Pass 1 sums what the step moves and checks it; nothing is written
+// before the whole step is known to fit.  Pass 2 pushes the returned pages,
+// pass 3 pops the taken ones; both spread the moved pages (not the requests)
+// over the threads, by a search in the scanned counts.
+// NOTOKENS: the tokens' slots are left to k_map_tokens.
+template <bool NOTOKENS>
+__global__ __launch_bounds__(kMapThreads) void k_page_map(MapArgs a) {
+    __shared__ int wave_sum[kMapThreads / 64];
+    __shared__ int upto[kMapThreads];
+    __shared__ int first[kMapThreads];
+    __shared__ unsigned long long sum64[3];
+    __shared__ int bad;
+    const int tid = threadIdx.x;
+    const int n_free = *a.n_free;
+    const int64_t cap = (int64_t)a.table_stride * a.page_size;
+    if (tid < 3) sum64[tid] = 0;
+    if (tid == 0) bad = n_free < 0 || n_free > a.n_pages;
+    __syncthreads();
+
+    // pass 1: totals, in 64 bits (any lengths may stand there)
+    unsigned long long ret = 0, take = 0, grow = 0;
+    bool wrong = false;
+    for (int r = tid; r < a.n_req; r += kMapThreads) {
+        const MapReq q = map_req(a, r);
+        wrong |= q.old_len < 0 || q.new_len < 0 || q.old_len > cap || q.new_len > cap;
+        ret += (unsigned)q.ret();
+        take += (unsigned)q.take();
+        grow += (unsigned)q.grow();
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        ret += __shfl_xor(ret, d);
+        take += __shfl_xor(take, d);
+        grow += __shfl_xor(grow, d);
+    }
+    if ((tid & 63) == 0) {
+        atomicAdd(&sum64[0], ret);
+        atomicAdd(&sum64[1], take);
+        atomicAdd(&sum64[2], grow);
+    }
+    if (wrong) bad = 1;
+    __syncthreads();
+    if (tid == 0 && ((int64_t)sum64[0] > (int64_t)a.n_pages - n_free || sum64[2] > (unsigned long long)a.max_tokens))
+        bad = 1;
+    __syncthreads();
+    const int n_ret = bad ? 0 : (int)sum64[0];
+
+    // the ids to be returned are checked before one of them is pushed
+    if (n_ret) {
+        for (int base = 0; base < a.n_req; base += kMapThreads) {
+            const MapReq q = map_req(a, base + tid);
+            int total;
+            const int up = block_scan(q.ret(), wave_sum, &total);
+            upto[tid] = up;
+            first[tid] = q.want - (up - q.ret());
+            __syncthreads();
+            for (int j = tid; j < total; j += kMapThreads) {
+                const int r = upper_bound(upto, kMapThreads, j);
+                const int id = a.table[(int64_t)(base + r) * a.table_stride + first[r] + j];
+                if (id < 0 || id >= a.n_pages) bad = 1;
+            }
+            __syncthreads();
+        }
+    }
+    const int status = bad ? 2 : (int64_t)sum64[1] > (int64_t)n_free + n_ret ? 1 : 0;
+
+    if (status) {   // nothing moves
+        for (int r = tid; r <= a.n_req; r += kMapThreads) {
+            a.cu_new[r] = 0;
+            if (r < a.n_req) a.len_out[r] = a.len_old[r];
+        }
+        if (!NOTOKENS)
+            for (int t = tid; t < a.max_tokens; t += kMapThreads) a.slots[t] = a.positions[t] = -1;
+        if (tid == 0) {
+            *a.n_free_out = n_free;
+            *a.status = status;
+        }
+        return;
+    }
+
+    // pass 2: returned pages onto the stack
+    if (n_ret) {
+        for (int base = 0, done = 0; base < a.n_req; base += kMapThreads) {
+            const MapReq q = map_req(a, base + tid);
+            int total;
+            const int up = block_scan(q.ret(), wave_sum, &total);
+            upto[tid] = up;
+            first[tid] = q.want - (up - q.ret());
+            __syncthreads();
+            for (int j = tid; j < total; j += kMapThreads) {
+                const int r = upper_bound(upto, kMapThreads, j);
+                a.free_pages[n_free + done + j] =
+                    a.table[(int64_t)(base + r) * a.table_stride + first[r] + j];
+            }
+            done += total;
+            __syncthreads();
+        }
+    }
+    const int top = n_free + n_ret;
+
+    // pass 3: taken pages off the stack's top; lengths, offsets, tokens
+    int taken = 0, grown = 0;
+    for (int base = 0; base < a.n_req; base += kMapThreads) {
+        const int rr = base + tid;
+        const MapReq q = map_req(a, rr);
+        int total;
+        int up = block_scan(q.take(), wave_sum, &total);
+        upto[tid] = up;
+        first[tid] = q.held - (up - q.take());
+        __syncthreads();
+        for (int j = tid; j < total; j += kMapThreads) {
+            const int r = upper_bound(upto, kMapThreads, j);
+            a.table[(int64_t)(base + r) * a.table_stride + first[r] + j] = a.free_pages[top - 1 - taken - j];
+        }
+        taken += total;
+        __syncthreads();
+        up = block_scan(q.grow(), wave_sum, &total);
+        if (rr < a.n_req) {
+            a.cu_new[rr] = grown + up - q.grow();
+            a.len_out[rr] = q.new_len;
+        }
+        if (!NOTOKENS) {
+            upto[tid] = up;
+            first[tid] = q.old_len - (up - q.grow());
+            __syncthreads();
+            for (int j = tid; j < total; j += kMapThreads) {
+                const int r = upper_bound(upto, kMapThreads, j);
+                map_token(a, grown + j, base + r, first[r] + j);
+            }
+        }
+        grown += total;
+        __syncthreads();
+    }
+    if (!NOTOKENS)
+        for (int t = grown + tid; t < a.max_tokens; t += kMapThreads) a.slots[t] = a.positions[t] = -1;
+    if (tid == 0) {
+        a.cu_new[a.n_req] = grown;
+        *a.n_free_out = top - taken;
+        *a.status = 0;
+    }
+}
+
+// Slots and positions of many tokens, after k_page_map<true>.
+__global__ __launch_bounds__(256) void k_map_tokens(MapArgs a) {
+    const int n = a.n_req, total = a.cu_new[n];
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < a.max_tokens; t += (int64_t)gridDim.x * 256) {
+        if (t >= total) {
+            a.slots[t] = a.positions[t] = -1;
+            continue;
+        }
+        // cu_new[0] = 0: the request is the last with cu_new <= t
+        const int r = upper_bound(a.cu_new, n + 1, (int)t) - 1;
+        const int grow = a.cu_new[r + 1] - a.cu_new[r];
+        map_token(a, (int)t, r, a.len_out[r] - grow + (int)t - a.cu_new[r]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Codes and scales
+// ---------------------------------------------------------------------------
+
+constexpr int kScaleMin = -100, kScaleMax = 120;   // exponents of a scale
+
+template <int FMT> struct Code;   // FMT: VKV_DTYPE_E4M3 or VKV_DTYPE_I8
+
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+__device__ __forceinline__ int exponent_of(float scale) {
+    const int e = (int)((__float_as_uint(scale) >> 23) & 255) - 127;
+    return min(max(e, kScaleMin), kScaleMax);
+}
+
+// Least e with amax <= largest code * 2^e.  The largest codes are 448 =
+// 1.75 * 2^8 and 127 = 1.984375 * 2^6, so e is the exponent of amax less 8 or
+// 6, and one more where the mantissa is larger.  A power of two, so that a
+// value in units of the scale is exact and only its rounding to a code loses
+// anything, and so that codes move to a larger scale without a second error
+// but for what falls below the smallest step.
+template <int FMT> __device__ __forceinline__ int scale_exponent(float amax) {
+    const unsigned b = __float_as_uint(amax);
+    const int x = (int)(b >> 23) - 127, m = (int)(b & 0x7fffff);
+    const int e = FMT == VKV_DTYPE_E4M3 ? x - 8 + (m > 0x600000) : x - 6 + (m > 0x7e0000);
+    return min(max(e, kScaleMin), kScaleMax);
+}
+
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= FLT_MAX; }
+
+// four values in units of the scale to four codes (nearest, ties to even)
+template <int FMT> __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
+    if constexpr (FMT == VKV_DTYPE_E4M3) {
+        const float nan = __builtin_nanf("");
+        a = is_finite(a) ? a : nan;
+        b = is_finite(b) ? b : nan;
+        c = is_finite(c) ? c : nan;
+        d = is_finite(d) ? d : nan;
+        unsigned r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+    } else {
+        auto one = [](float x) -> unsigned {
+            x = x == x ? x : 0.0f;
+            x = fminf(fmaxf(rintf(x), -127.0f), 127.0f);
+            return (unsigned)(int)x & 255u;
+        };
+        return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+    }
+}
+
+template <int FMT> __device__ __forceinline__ void unpack4(unsigned w, float v[4]) {
+    if constexpr (FMT == VKV_DTYPE_E4M3) {
+        v[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0);
+        v[1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);
+        v[2] = __builtin_amdgcn_cvt_f32_fp8(w, 2);
+        v[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
+    } else {
+        v[0] = (float)(int8_t)(w & 255);
+        v[1] = (float)(int8_t)(w >> 8 & 255);
+        v[2] = (float)(int8_t)(w >> 16 & 255);
+        v[3] = (float)(int8_t)(w >> 24);
+    }
+}
+
+// codes at a scale 2^k times smaller than the new one, k > 0
+template <int FMT> __device__ __forceinline__ unsigned rescale4(unsigned w, float down) {
+    float v[4];
+    unpack4<FMT>(w, v);
+    return pack4<FMT>(v[0] * down, v[1] * down, v[2] * down, v[3] * down);
+}
+
+// ---------------------------------------------------------------------------
+// Append
+// ---------------------------------------------------------------------------
+
+template <typename T> __device__ __forceinline__ float to_f32(T x) { return (float)x; }
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+
+// One work group per new token that opens its page's run of tokens, and four
+// (K or V, head) units; the other tokens' work groups end at once.  A wave
+// owns one unit of the page: largest magnitude of the run's rows, the scale
+// they need, then the codes of every 16-token block of the page that changes.
+// Lane (g, c) of a block: K rows 4 j + g, dims [c D/16, (c + 1) D/16); V rows
+// 4 g + j, dims 16 t + c, which is the block's stored order.
+template <typename T, int FMT, int D>
+__global__ __launch_bounds__(256) void k_pages_append(AppendPagesArgs a) {
+    constexpr int N = D / 16;
+    __shared__ int win[256];    // last token of the run for each slot of the page, -1: none
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int S = a.page_size;
+    const int slot = a.slots[t];
+    if (slot < 0 || slot >= a.n_slots) return;
+    const int page = slot / S;
+    if (t > 0) {
+        const int before = a.slots[t - 1];
+        if (before >= 0 && before < a.n_slots && before / S == page) return;
+    }
+    if (tid < S) win[tid] = -1;
+    __syncthreads();
+    for (int i0 = t;; i0 += 256) {
+        const int i = i0 + tid;
+        const int s = i < a.n_tokens ? a.slots[i] : -1;
+        const bool in = s >= 0 && s < a.n_slots && s / S == page;
+        // the run ends at the first token of another page
+        __shared__ int end;
+        if (tid == 0) end = i0 + 256;
+        __syncthreads();
+        if (!in) atomicMin(&end, i);
+        __syncthreads();
+        const int stop = end;
+        if (i < stop) atomicMax(&win[s - page * S], i);
+        __syncthreads();
+        if (stop < i0 + 256) break;
+    }
+    const int unit = blockIdx.y * 4 + (tid >> 6);
+    if (unit >= 2 * a.n_kv_heads) return;
+    const bool is_v = unit >= a.n_kv_heads;
+    const int head = is_v ? unit - a.n_kv_heads : unit;
+    const int g = lane >> 4, c = lane & 15;
+    const T *src = (const T *)(is_v ? a.v : a.k) + head * D + (is_v ? c : c * N);
+    const int step = is_v ? 16 : 1;      // between a lane's dims
+    const int64_t ph = (int64_t)page * a.n_kv_heads + head;
+    uint8_t *codes = (is_v ? a.v_codes : a.k_codes) + ph * ((int64_t)S * D);
+    float *scale = (is_v ? a.v_scale : a.k_scale) + ph;
+
+    auto row_of = [&](int b, int j) { return win[16 * b + (is_v ? 4 * g + j : 4 * j + g)]; };
+    float amax = 0.0f;
+    for (int b = 0; b < S / 16; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = row_of(b, j);
+            if (i < 0) continue;
+            const T *p = src + (int64_t)i * a.row_stride;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const float x = to_f32(p[n * step]);
+                amax = fmaxf(amax, is_finite(x) ? fabsf(x) : 0.0f);
+            }
+        }
+    amax = wave_max(amax);
+    int e = scale_exponent<FMT>(amax);
+    // a page begins with its slot 0: what it held before does not count
+    const bool fresh = win[0] >= 0;
+    float down = 1.0f;
+    if (!fresh) {
+        const int old = exponent_of(*scale);
+        if (e > old) down = exp2_int(max(old - e, -126)); else e = old;
+    }
+    const bool grown = down != 1.0f;
+    const float inv = exp2_int(-e);
+    if (lane == 0) *scale = exp2_int(e);
+
+    for (int b = 0; b < S / 16; ++b) {
+        bool any = false;
+        int rows[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            rows[j] = row_of(b, j);
+            any |= rows[j] >= 0;
+        }
+        if (!any && !grown) continue;
+        float x[4][N];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const T *p = src + (int64_t)max(rows[j], 0) * a.row_stride;
+            if (rows[j] >= 0)
+#pragma unroll
+                for (int n = 0; n < N; ++n) x[j][n] = to_f32(p[n * step]) * inv;
+        }
+        if (!is_v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                unsigned *dst = (unsigned *)(codes + (int64_t)(16 * b + 4 * j + g) * D + c * N);
+#pragma unroll
+                for (int n = 0; n < N / 4; ++n) {
+                    if (rows[j] >= 0)
+                        dst[n] = pack4<FMT>(x[j][4 * n], x[j][4 * n + 1], x[j][4 * n + 2], x[j][4 * n + 3]);
+                    else if (grown)
+                        dst[n] = rescale4<FMT>(dst[n], down);
+                }
+            }
+        } else {
+            unsigned *dst = (unsigned *)(codes + (int64_t)b * 16 * D) + (c * 4 + g) * N;
+            unsigned mask = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mask |= rows[j] >= 0 ? 255u << 8 * j : 0u;
+            if (mask != 0 || grown) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    unsigned w = 0;
+                    if (mask != 0xffffffffu) {
+                        w = dst[n];
+                        if (grown) w = rescale4<FMT>(w, down);
+                    }
+                    const unsigned y = pack4<FMT>(rows[0] >= 0 ? x[0][n] : 0.0f, rows[1] >= 0 ? x[1][n] : 0.0f,
+                                                  rows[2] >= 0 ? x[2][n] : 0.0f, rows[3] >= 0 ? x[3][n] : 0.0f);
+                    dst[n] = (w & ~mask) | (y & mask);
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Single-query attention
+// ---------------------------------------------------------------------------
+
+// four codes to f16, exactly
+template <int FMT> __device__ __forceinline__ void codes_f16(unsigned w, half2_t &lo, half2_t &hi) {
+    if constexpr (FMT == VKV_DTYPE_E4M3) {
+        lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+    } else {
+        // 0x6400 | u is 1024 + u in f16, with u = code + 128
+        const unsigned u = w ^ 0x80808080u;
+        const unsigned a = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+        const unsigned b = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+        const half2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
+        lo = __builtin_bit_cast(half2_t, a) - off;
+        hi = __builtin_bit_cast(half2_t, b) - off;
+    }
+}
+
+template <int FMT> __device__ __forceinline__ half8_t codes8(unsigned w0, unsigned w1) {
+    half2_t a, b, c, d;
+    codes_f16<FMT>(w0, a, b);
+    codes_f16<FMT>(w1, c, d);
+    return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// the other half of a lane's 16-lane row: lane n and n ^ 8
+__device__ __forceinline__ float row_ror8(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
+}
+
+// over the four 16-lane rows of a wave
+__device__ __forceinline__ float rows_max(float x) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ float lane_value(float x, int lane) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
+}
+
+// What a row attends to: keys [lo, len), none where len <= 0.
+struct Span {
+    int lo, len;
+    bool bad;     // a length that the call's bounds or the table do not hold
+};
+__device__ __forceinline__ Span row_span(const PagedAttnArgs &a, int row) {
+    Span s;
+    s.len = a.lens[row];
+    s.bad = s.len > a.max_len;
+    s.lo = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
+    return s;
+}
+
+template <typename T> __device__ __forceinline__ T from_f32(float x) { return (T)x; }
+
+constexpr int kAttnWaves = 4;
+
+// A work group is 4 waves on (row, kv head, up to 8 query heads, chunk of
+// keys); wave w takes the chunk's 32-key steps w, w + 4, ...
+//
+// Both products run on v_mfma_f32_16x16x32_f16, whose f16 operands hold the
+// 8-bit codes exactly.  S^T = K Q^T: 16 keys by 16 columns, and O^T = V^T P:
+// 16 dims by 16 columns.  A column is a query head in the lower 8 and the
+// same head's remainder in the upper 8: q (and p) are split as hi + lo /
+// 2048 with hi and lo in f16, 22 bits together, so the result keeps the
+// accuracy of 32-bit operands without a second product: the columns would
+// else be empty for up to 8 heads per kv head.  q is first put into [1, 2)
+// by a power of two per head.
+//
+// The rows of S^T that a lane holds (keys 4 g + i of each of the step's two
+// 16-key blocks) are the keys it supplies to the second product, so P goes
+// from one product to the next in the lane's own registers.
+template <typename T, int FMT, int D, bool DIRECT>
+__global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a) {
+    constexpr int NL = D / 64;    // 16-byte loads per lane and 16-key block, K or V
+    constexpr int NM = D / 32;    // MFMAs per 16-key block of scores
+    constexpr int NT = D / 16;    // 16-dim tiles of the output
+    __shared__ float lds_o[kAttnWaves][8][D];
+    __shared__ float lds_ml[kAttnWaves][8][2];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int group = a.n_q_heads / a.n_kv_heads, tiles = (group + 7) / 8;
+    const int kvh = blockIdx.x % a.n_kv_heads;
+    const int tile = blockIdx.x / a.n_kv_heads % tiles;
+    const int row = blockIdx.x / (a.n_kv_heads * tiles);
+    const int chunk = blockIdx.y;
+    const int heads = min(group - 8 * tile, 8);
+    const int head0 = kvh * group + 8 * tile;
+
+    const Span sp = row_span(a, row);
+    const int base = sp.lo & ~31;
+    const int k0 = base + chunk * a.chunk;
+    if (sp.bad || k0 >= sp.len) {
+        if (DIRECT) {
+            T *out = (T *)a.out + (int64_t)row * a.out_stride + (int64_t)head0 * D;
+            const float v = sp.bad ? __builtin_nanf("") : 0.0f;
+            for (int i = tid; i < heads * D; i += 64 * kAttnWaves) out[i] = from_f32<T>(v);
+        }
+        return;
+    }
+    const int k1 = min(sp.len, k0 + a.chunk);
+
+    // The chunk's 16-key blocks, one per lane (chunk <= 1024): index of the
+    // block in the layer, and its page's scales.
+    const int kb = k0 + 16 * lane;
+    const bool mine = kb < k1;
+    int id = 0;
+    if (mine) id = a.table[(int64_t)row * a.table_stride + kb / a.page_size];
+    const bool off = id < 0 || id >= a.n_pages;
+    if (off) id = 0;
+    const bool bad_page = __any(mine && off);
+    const int ph = id * a.n_kv_heads + kvh;
+    const int blk = ph * (a.page_size / 16) + kb % a.page_size / 16;
+    const float ks = a.k_scale[ph];
+    float vs = mine ? a.v_scale[ph] : 0.0f;
+    // V's codes are weighted by their scale over the chunk's largest: powers
+    // of two, so nothing is rounded
+    float vref = wave_max(vs);
+    vs *= vref > 0.0f ? 1.0f / vref : 0.0f;
+
+    // this lane's column of Q: dims 64 i + 16 g + 8 m + [0, 8) of MFMA 2 i + m
+    const int col_head = head0 + min(n & 7, heads - 1);
+    const T *q = (const T *)a.q + (int64_t)row * a.q_stride + (int64_t)col_head * D;
+    float qv[NM][8];
+    float qmax = 0.0f;
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            qv[m][i] = to_f32(q[64 * (m / 2) + 16 * g + 8 * (m % 2) + i]);
+            qmax = fmaxf(qmax, fabsf(qv[m][i]));
+        }
+    qmax = rows_max(qmax);
+    const int eq = qmax > 0.0f && is_finite(qmax) ? max((int)(__float_as_uint(qmax) >> 23) - 127, -126) : 0;
+    half8_t qf[NM];
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = ldexpf(qv[m][i], -eq);
+            const _Float16 hi = (_Float16)x;
+            qf[m][i] = n < 8 ? hi : (_Float16)((x - (float)hi) * 2048.0f);
+        }
+    const float qfac = ldexpf(a.scale * kLog2e, eq);
+
+    floatx4 o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] = floatx4{0, 0, 0, 0};
+    float m_run = -INFINITY, l = 0.0f;
+
+    const uint8_t *k_lane = a.k_codes + n * D + 16 * g;
+    const uint8_t *v_lane = a.v_codes + (n * 4 + g) * NT * 4;
+    uint4 kr[2][NL], vr[2][NL];
+    auto load = [&](int s) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int at = min((s - k0) / 16 + b, (k1 - 1 - k0) / 16);
+            const int64_t byte = (int64_t)__builtin_amdgcn_readlane(blk, at) * (16 * D);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                kr[b][i] = *(const uint4 *)(k_lane + byte + 64 * i);
+                vr[b][i] = *(const uint4 *)(v_lane + byte + 16 * i);
+            }
+        }
+    };
+    for (int s = k0 + 32 * wave; s < k1; s += 32 * kAttnWaves) {
+        load(s);
+        floatx4 sc[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            floatx4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(kr[b][i].x, kr[b][i].y), qf[2 * i], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(kr[b][i].z, kr[b][i].w), qf[2 * i + 1], acc, 0, 0, 0);
+            }
+            const float f = qfac * lane_value(ks, (s - k0) / 16 + b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = acc[i], y = row_ror8(x);
+                sc[b][i] = ((n < 8 ? x : y) + (n < 8 ? y : x) * (1.0f / 2048.0f)) * f;
+            }
+        }
+        if (s < sp.lo || s + 32 > k1) {
+            // the first and the last step: keys outside the span weigh
+            // nothing, and their V codes (which may be anything) become 0
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                unsigned keep = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = s + 16 * b + 4 * g + i;
+                    const bool in = key >= sp.lo && key < k1;
+                    sc[b][i] = in ? sc[b][i] : -INFINITY;
+                    keep |= in ? 255u << 8 * i : 0u;
+                }
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    vr[b][i].x &= keep;
+                    vr[b][i].y &= keep;
+                    vr[b][i].z &= keep;
+                    vr[b][i].w &= keep;
+                }
+            }
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i / 4][i % 4]);
+        mx = rows_max(mx);
+        // the running maximum moves only when it is passed by 2^8: p <= 256
+        if (__any(mx > m_run + 8.0f)) {
+            const float m_new = fmaxf(m_run, mx);
+            const float f = m_new > -INFINITY ? exp2f(m_run - m_new) : 1.0f;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t] *= f;
+            m_run = m_new;
+        }
+        const float m_use = m_run > -INFINITY ? m_run : 0.0f;
+        half8_t p8;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const float w = lane_value(vs, (s - k0) / 16 + b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = exp2f(sc[b][i] - m_use);
+                l += p;
+                const float x = p * w;
+                const _Float16 hi = (_Float16)x;
+                p8[4 * b + i] = n < 8 ? hi : (_Float16)((x - (float)hi) * 2048.0f);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint4 va = vr[0][t / 4], vb = vr[1][t / 4];
+            const unsigned wa = t % 4 == 0 ? va.x : t % 4 == 1 ? va.y : t % 4 == 2 ? va.z : va.w;
+            const unsigned wb = t % 4 == 0 ? vb.x : t % 4 == 1 ? vb.y : t % 4 == 2 ? vb.z : vb.w;
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(wa, wb), p8, o[t], 0, 0, 0);
+        }
+    }
+
+    // the four waves' parts meet in LDS
+    l = rows_sum(l);
+    if (n < 8 && g == 0) {
+        lds_ml[wave][n][0] = m_run;
+        lds_ml[wave][n][1] = l;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = o[t][i], y = row_ror8(x);
+            if (n < 8) lds_o[wave][n][16 * t + 4 * g + i] = (x + y * (1.0f / 2048.0f)) * vref;
+        }
+    __syncthreads();
+    for (int i = tid; i < heads * D; i += 64 * kAttnWaves) {
+        const int h = i / D, d = i % D;
+        float m = lds_ml[0][h][0];
+#pragma unroll
+        for (int w = 1; w < kAttnWaves; ++w) m = fmaxf(m, lds_ml[w][h][0]);
+        float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; ++w) {
+            const float f = lds_ml[w][h][0] > -INFINITY ? exp2f(lds_ml[w][h][0] - m) : 0.0f;
+            sum += f * lds_ml[w][h][1];
+            acc += f * lds_o[w][h][d];
+        }
+        if (bad_page) acc = sum = __builtin_nanf("");
+        if (DIRECT) {
+            T *out = (T *)a.out + (int64_t)row * a.out_stride + (int64_t)head0 * D;
+            out[i] = from_f32<T>(sum != 0.0f ? acc / sum : 0.0f);
+        } else {
+            const int64_t part = ((int64_t)row * a.n_q_heads + head0 + h) * a.n_chunks + chunk;
+            a.part_o[part * D + d] = acc;
+            if (d == 0) {
+                a.part_ml[part * 2] = m;
+                a.part_ml[part * 2 + 1] = sum;
+            }
+        }
+    }
+}
+
+// Joins the chunks of a (row, query head); D threads, chunks in rising order.
+template <typename T, int D>
+__global__ __launch_bounds__(D) void k_paged_merge(PagedAttnArgs a) {
+    const int head = blockIdx.x % a.n_q_heads, row = blockIdx.x / a.n_q_heads;
+    const int d = threadIdx.x;
+    T *out = (T *)a.out + (int64_t)row * a.out_stride + (int64_t)head * D + d;
+    const Span sp = row_span(a, row);
+    if (sp.bad || sp.len <= 0) {
+        *out = from_f32<T>(sp.bad ? __builtin_nanf("") : 0.0f);
+        return;
+    }
+    const int n = min(a.n_chunks, (sp.len - (sp.lo & ~31) + a.chunk - 1) / a.chunk);
+    const int64_t part = (int64_t)blockIdx.x * a.n_chunks;
+    const float *ml = a.part_ml + part * 2;
+    float m = -INFINITY;
+    for (int i = 0; i < n; ++i) m = fmaxf(m, ml[2 * i]);
+    float sum = 0.0f, acc = 0.0f;
+    for (int i = 0; i < n; ++i) {
+        const float f = ml[2 * i] == -INFINITY ? 0.0f : exp2f(ml[2 * i] - m);
+        sum += f * ml[2 * i + 1];
+        acc += f * a.part_o[(part + i) * D + d];
+    }
+    *out = from_f32<T>(sum != 0.0f ? acc / sum : 0.0f);
+}
+
+template <typename T, int FMT, int D> hipError_t attn_launch(const PagedAttnArgs &a, hipStream_t st) {
+    const int tiles = (a.n_q_heads / a.n_kv_heads + 7) / 8;
+    const dim3 grid((unsigned)(a.n_rows * a.n_kv_heads * tiles), (unsigned)a.n_chunks);
+    if (a.n_chunks == 1) {
+        k_paged_attn<T, FMT, D, true><<<grid, 64 * kAttnWaves, 0, st>>>(a);
+    } else {
+        k_paged_attn<T, FMT, D, false><<<grid, 64 * kAttnWaves, 0, st>>>(a);
+        k_paged_merge<T, D><<<(unsigned)(a.n_rows * a.n_q_heads), D, 0, st>>>(a);
+    }
+    return hipGetLastError();
+}
+
+template <typename T, int FMT, int D> hipError_t append_launch(const AppendPagesArgs &a, hipStream_t st) {
+    const dim3 grid((unsigned)a.n_tokens, (unsigned)((2 * a.n_kv_heads + 3) / 4));
+    k_pages_append<T, FMT, D><<<grid, 256, 0, st>>>(a);
+    return hipGetLastError();
+}
+
+// f(type tag, format constant, head dim constant) for a call's types
+template <typename F> hipError_t by_types(int dtype, int code, int head_dim, F f) {
+    auto dim = [&](auto t, auto c) {
+        if (head_dim == 64) return f(t, c, std::integral_constant<int, 64>{});
+        return f(t, c, std::integral_constant<int, 128>{});
+    };
+    auto fmt = [&](auto t) {
+        if (code == VKV_DTYPE_I8) return dim(t, std::integral_constant<int, VKV_DTYPE_I8>{});
+        return dim(t, std::integral_constant<int, VKV_DTYPE_E4M3>{});
+    };
+    if (dtype == VKV_DTYPE_F16) return fmt((_Float16)0);
+    if (dtype == VKV_DTYPE_BF16) return fmt((__bf16)0.0f);
+    return fmt(0.0f);
+}
+
+}  // namespace
+
+hipError_t launch_page_map(const MapArgs &a, hipStream_t st) {
+    if (a.max_tokens <= kMapInlineTokens) {
+        k_page_map<false><<<1, kMapThreads, 0, st>>>(a);
+    } else {
+        k_page_map<true><<<1, kMapThreads, 0, st>>>(a);
+        const int64_t wgs = ((int64_t)a.max_tokens + 255) / 256;
+        k_map_tokens<<<(unsigned)(wgs < 65536 ? wgs : 65536), 256, 0, st>>>(a);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_pages_append(int dtype, int code, int head_dim, const AppendPagesArgs &a, hipStream_t st) {
+    return by_types(dtype, code, head_dim, [&](auto t, auto c, auto d) {
+        return append_launch<decltype(t), decltype(c)::value, decltype(d)::value>(a, st);
+    });
+}
+
+hipError_t launch_paged_attn(int dtype, int code, int head_dim, const PagedAttnArgs &a, hipStream_t st) {
+    return by_types(dtype, code, head_dim, [&](auto t, auto c, auto d) {
+        return attn_launch<decltype(t), decltype(c)::value, decltype(d)::value>(a, st);
+    });
+}
+
+}  // namespace vkv

@@ -1,0 +1,480 @@
+// Causal attention of packed prompts on gfx950.
+//
+// Two launches.  k_prompt_pack turns each prompt's K and V, 64 keys and one kv
+// head at a time, into the operands of v_mfma_f32_32x32x16: 1 KiB pieces of
+// 16 bytes per lane, V transposed.  Every query tile of the prompt reads them
+// again, so the transposition, the split of f32 rows and the search for the
+// largest value are paid once per key instead of once per (key, query tile).
+// k_prompt_attn then streams them into LDS unchanged and keeps everything
+// else in registers.
+//
+// f32 rows are multiplied as hi + lo with both in f16 (x hi, lo = x - hi;
+// three products, the fourth is below f32's own rounding): the matrix cores'
+// f32 form runs at 1/16 of the f16 rate, the three f16 products at 1/3.  q is
+// scaled by a power of two per row, K and V per tile, to a largest magnitude
+// in [2^13, 2^14), so that lo keeps its 11 bits down to 2^-13 of it.
+#include <hip/hip_runtime.h>
+
+#include <cfloat>
+
+#include "vkv_serve.h"
+
+namespace vkv {
+namespace {
+
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kTile = kPromptKeys;
+constexpr int kTopExp = 13;     // scaled rows have their largest magnitude in [2^13, 2^14)
+constexpr int kPExp = 6;        // p <= 2^8 is scaled to <= 2^14
+
+// T: type of the rows; F32 rows become two f16 planes
+template <typename T> struct Operand {
+    typedef _Float16 elem;
+    static constexpr int planes = 1;
+};
+template <> struct Operand<float> {
+    typedef _Float16 elem;
+    static constexpr int planes = 2;
+};
+template <> struct Operand<__bf16> {
+    typedef __bf16 elem;
+    static constexpr int planes = 1;
+};
+
+template <typename E> __device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
+    if constexpr (std::is_same<E, __bf16>::value)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+template <typename E> struct Vec8 { typedef E type __attribute__((ext_vector_type(8))); };
+
+// eight values rounded to the operand type
+template <typename E> __device__ __forceinline__ uint4 round8(const float *x) {
+    typename Vec8<E>::type r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (E)x[i];
+    return __builtin_bit_cast(uint4, r);
+}
+
+// and what that leaves of them; nothing of what is not finite
+__device__ __forceinline__ uint4 rest8(const float *x) {
+    half8_t r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float hi = (float)(_Float16)x[i];
+        r[i] = (_Float16)(fabsf(hi) <= FLT_MAX ? x[i] - hi : 0.0f);
+    }
+    return __builtin_bit_cast(uint4, r);
+}
+
+template <typename T> __device__ __forceinline__ void load8(const T *p, float *x) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const auto v = __builtin_bit_cast(typename Vec8<T>::type, *(const uint4 *)p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+    }
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+    x = fabsf(x);
+    return x <= FLT_MAX ? x : 0.0f;
+}
+
+__device__ __forceinline__ int exponent(float amax) {
+    return amax > 0.0f ? max((int)(__float_as_uint(amax) >> 23) - 127, -100) : 0;
+}
+
+// the two halves of a wave
+__device__ __forceinline__ float halves_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+struct Prompt {
+    int seq, start, n, local;    // local: the slot's number among the prompt's own
+};
+
+// Prompt i's slots of `per` units begin at floor(cu[i] * mul / per) + i: at
+// least ceil(n_i * mul / per) of them lie before prompt i + 1's, so the place
+// of every slot follows from the offsets alone, without a sum over the
+// prompts.  Offsets are held to [0, n_tokens], whatever they are.
+__device__ __forceinline__ int offset_of(const PromptArgs &a, int i) { return min(max(a.cu[i], 0), a.n_tokens); }
+__device__ __forceinline__ bool find_prompt(const PromptArgs &a, int64_t slot, int mul, int per, Prompt &p) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = a.n_seq;
+    for (;;) {   // a 64th of the range is left at each turn
+        const int step = (hi - lo + 63) / 64;
+        const int i = lo + lane * step;
+        const bool le = i < hi && (int64_t)offset_of(a, min(i, a.n_seq)) * mul / per + i <= slot;
+        const int c = __popcll(__ballot(le));
+        if (c == 0) return false;
+        lo += (c - 1) * step;
+        hi = min(hi, lo + step);
+        if (step == 1) break;
+    }
+    p.seq = __builtin_amdgcn_readfirstlane(lo);
+    p.start = offset_of(a, p.seq);
+    p.n = max(offset_of(a, p.seq + 1) - p.start, 0);
+    p.local = (int)(slot - ((int64_t)p.start * mul / per + p.seq));
+    return true;
+}
+
+// A tile's operands: K, planes x [2 blocks of 32 keys][D/16][64 lanes] 16
+// bytes: lane (r, h) has key 32 kb + r, dims 16 m + 8 h + [0, 8).  V, planes x
+// [D/32][4 blocks of 16 keys][64 lanes]: lane (r, h) has dim 32 dt + r, keys
+// 16 u + 4 h + [0, 4) and 16 u + 8 + 4 h + [0, 4), the keys whose scores a
+// lane of half h holds.
+template <typename T, int D> constexpr int tile_bytes() { return Operand<T>::planes * 2 * kTile * D * 2; }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
+    typedef typename Operand<T>::elem E;
+    constexpr int NP = Operand<T>::planes;
+    constexpr int NS = kTile * D / 8 / 256;     // 16-byte pieces per thread, K or V
+    __shared__ float vt[kTile][D];
+    __shared__ float red[4][2];
+    __shared__ int odd;
+    const int tid = threadIdx.x;
+    const int head = blockIdx.y;
+    Prompt p;
+    if (!find_prompt(a, blockIdx.x, 1, kTile, p)) return;
+    const int key0 = p.local * kTile;
+    if (key0 >= p.n) return;
+    if (tid == 0) odd = 0;
+    __syncthreads();
+    const int64_t tile = (int64_t)head * a.n_tiles + blockIdx.x;
+
+    float kx[NS][8];
+    float kmax = 0.0f, vmax = 0.0f;
+    bool strange = false;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        const int piece = tid + 256 * s, l = piece & 63, m = (piece >> 6) % (D / 16), kb = (piece >> 6) / (D / 16);
+        const int key = key0 + 32 * kb + (l & 31);
+        if (key < p.n)
+            load8((const T *)a.k + (p.start + key) * a.k_stride + head * D + 16 * m + 8 * (l >> 5), kx[s]);
+        else
+            for (int i = 0; i < 8; ++i) kx[s][i] = 0.0f;
+        // V by rows into LDS
+        const int row = piece / (D / 8), d = piece % (D / 8) * 8;
+        float x[8];
+        if (key0 + row < p.n)
+            load8((const T *)a.v + (p.start + key0 + row) * a.v_stride + head * D + d, x);
+        else
+            for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // a key without weight must not reach the output, and 0 times
+            // what is not finite would: such values are left to k_prompt_attn
+            const bool fine = fabsf(x[i]) <= FLT_MAX;
+            strange |= !fine;
+            vt[row][d + i] = fine ? x[i] : 0.0f;
+            kmax = fmaxf(kmax, finite_abs(kx[s][i]));
+            vmax = fmaxf(vmax, finite_abs(x[i]));
+        }
+    }
+    if (strange) odd = 1;
+    int ek = kTopExp, ev = kTopExp;
+    if constexpr (NP == 2) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            kmax = fmaxf(kmax, __shfl_xor(kmax, d));
+            vmax = fmaxf(vmax, __shfl_xor(vmax, d));
+        }
+        if ((tid & 63) == 0) {
+            red[tid >> 6][0] = kmax;
+            red[tid >> 6][1] = vmax;
+        }
+        __syncthreads();
+        ek = exponent(fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0])));
+        ev = exponent(fmaxf(fmaxf(red[0][1], red[1][1]), fmaxf(red[2][1], red[3][1])));
+    } else {
+        __syncthreads();
+    }
+    uint4 *out = (uint4 *)(a.data + tile * tile_bytes<T, D>());
+    constexpr int PLANE = kTile * D / 8;        // 16-byte pieces of a plane
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        const int piece = tid + 256 * s;
+        if constexpr (NP == 2) {
+            for (int i = 0; i < 8; ++i) kx[s][i] = ldexpf(kx[s][i], kTopExp - ek);
+            out[PLANE + piece] = rest8(kx[s]);
+        }
+        out[piece] = round8<E>(kx[s]);
+        const int l = piece & 63, u = (piece >> 6) & 3, dt = piece >> 8;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = 16 * u + (i >= 4 ? 8 : 0) + 4 * (l >> 5) + (i & 3);
+            x[i] = vt[key][32 * dt + (l & 31)];
+            if constexpr (NP == 2) x[i] = ldexpf(x[i], kTopExp - ev);
+        }
+        if constexpr (NP == 2) out[3 * PLANE + piece] = rest8(x);
+        out[NP * PLANE + piece] = round8<E>(x);
+    }
+    if (tid == 0) {
+        int32_t *info = a.info + tile * 4;
+        info[0] = ek;
+        info[1] = ev;
+        info[2] = odd;
+        info[3] = 0;
+    }
+}
+
+// A work group: 8 waves on 256 rows of one (prompt, kv head), a row being
+// (token, query head of the kv head), so the heads that share K and V read one
+// copy of them in LDS.  Wave w owns rows 32 w + [0, 32) as the columns of S^T =
+// K Q^T and O^T = V^T P^T; a lane's scores are the keys it supplies to the
+// second product, so P stays in its registers.  Key tiles are double-buffered
+// in LDS by loads that go there without registers.
+template <typename T, int D>
+__global__ __launch_bounds__(2 * kPromptRows) void k_prompt_attn(PromptArgs a) {
+    typedef typename Operand<T>::elem E;
+    constexpr int NP = Operand<T>::planes;
+    constexpr int NM = D / 16, ND = D / 32;
+    constexpr int BYTES = tile_bytes<T, D>();
+    constexpr int PLANE = kTile * D * 2;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5;
+    const int group = a.n_q_heads / a.n_kv_heads;
+    const int head = blockIdx.x % a.n_kv_heads;
+    // the later tiles of a prompt have the most keys: they go first
+    const int64_t slot = a.n_slots - 1 - blockIdx.x / a.n_kv_heads;
+    Prompt p;
+    if (!find_prompt(a, slot, group, kPromptRows, p)) return;
+    const int64_t rows = (int64_t)p.n * group;
+    const int64_t row0 = (int64_t)p.local * kPromptRows;
+    if (row0 >= rows) return;
+
+    const int64_t wrow = row0 + 32 * wave;
+    const bool busy = wrow < rows;
+    const int64_t row = wrow + (lane & 31);
+    const int64_t row_in = row < rows ? row : rows - 1;
+    const int token = (int)(row_in / group), hq = (int)(row_in % group);
+    const int t_first = (int)((busy ? wrow : rows - 1) / group);
+    const int t_last = (int)((wrow + 31 < rows ? wrow + 31 : rows - 1) / group);
+    const int wg_first = (int)(row0 / group);
+    const int wg_last = (int)((row0 + kPromptRows - 1 < rows ? row0 + kPromptRows - 1 : rows - 1) / group);
+    const int kt0 = a.window > 0 && wg_first >= a.window ? (wg_first - a.window + 1) / kTile : 0;
+    const int kt1 = wg_last / kTile;
+    const int64_t tile0 = (int64_t)head * a.n_tiles + p.start / kTile + p.seq;
+
+    auto fetch = [&](int kt, int buf) {
+        const uint8_t *src = a.data + (tile0 + kt) * BYTES + tid * 16;
+#pragma unroll
+        for (int i = 0; i < BYTES / (2 * kPromptRows * 16); ++i)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) unsigned *)(src + i * (2 * kPromptRows * 16)),
+                (__attribute__((address_space(3))) unsigned *)(lds + buf * BYTES + i * (2 * kPromptRows * 16) + wave * 1024),
+                16, 0, 0);
+    };
+    fetch(kt0, 0);
+
+    // this lane's column of Q: dims 16 m + 8 half + [0, 8)
+    uint4 qf[NP][NM];
+    float qfac = fabsf(a.scale) * kLog2e;
+    {
+        const T *q = (const T *)a.q + (p.start + token) * a.q_stride + (head * group + hq) * D + 8 * half;
+        float x[NM][8];
+        float qmax = 0.0f;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            load8(q + 16 * m, x[m]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (a.scale < 0.0f) x[m][i] = -x[m][i];
+                qmax = fmaxf(qmax, finite_abs(x[m][i]));
+            }
+        }
+        if constexpr (NP == 2) {
+            const int e = exponent(halves_max(qmax));
+            qfac = ldexpf(qfac, e - kTopExp);
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[m][i] = ldexpf(x[m][i], kTopExp - e);
+                qf[1][m] = rest8(x[m]);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < NM; ++m) qf[0][m] = round8<E>(x[m]);
+    }
+
+    floatx16 o[ND];
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    float m_run = -INFINITY, l = 0.0f;
+    int ev_ref = -1000;
+
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+    __syncthreads();
+    for (int kt = kt0; kt <= kt1; ++kt) {
+        const int buf = (kt - kt0) & 1;
+        if (kt < kt1) fetch(kt + 1, buf ^ 1);
+        const int key0 = kt * kTile;
+        const bool seen = busy && key0 <= t_last && (a.window <= 0 || key0 + kTile > t_first - a.window + 1);
+        if (seen) {
+            const uint8_t *kl = lds + buf * BYTES + lane * 16, *vl = kl + NP * PLANE;
+            const int32_t *info = a.info + (tile0 + kt) * 4;
+            const int ek = info[0], ev = info[1], odd = info[2];
+            const float f = fmaxf(NP == 2 ? ldexpf(qfac, ek - kTopExp) : qfac, FLT_MIN);
+            floatx16 s[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+                for (int m = 0; m < NM; ++m) {
+                    const uint4 hi = *(const uint4 *)(kl + (kb * NM + m) * 1024);
+                    s[kb] = mfma<E>(hi, qf[0][m], s[kb]);
+                    if constexpr (NP == 2) {
+                        const uint4 lo = *(const uint4 *)(kl + PLANE + (kb * NM + m) * 1024);
+                        s[kb] = mfma<E>(hi, qf[1][m], s[kb]);
+                        s[kb] = mfma<E>(lo, qf[0][m], s[kb]);
+                    }
+                }
+            }
+            if (key0 + kTile - 1 > t_first || (a.window > 0 && key0 <= t_last - a.window)) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3);
+                        const bool in = key <= token && (a.window <= 0 || key > token - a.window);
+                        s[kb][i] = in ? s[kb][i] : -INFINITY;
+                    }
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
+            mx = halves_max(mx) * f;
+            // the running maximum moves only when it is passed by 2^8
+            if (__any(mx > m_run + 8.0f)) {
+                const float m_new = fmaxf(m_run, mx);
+                const float g = m_new > -INFINITY ? exp2f(m_run - m_new) : 1.0f;
+                l *= g;
+#pragma unroll
+                for (int t = 0; t < ND; ++t) o[t] *= g;
+                m_run = m_new;
+            }
+            float pfac = 1.0f;
+            if constexpr (NP == 2) {
+                if (ev > ev_ref) {
+                    const float g = ldexpf(1.0f, max(ev_ref - ev, -300));
+#pragma unroll
+                    for (int t = 0; t < ND; ++t) o[t] *= g;
+                    ev_ref = ev;
+                }
+                pfac = ldexpf(1.0f, kPExp + ev - ev_ref);
+            }
+            const float m_use = m_run > -INFINITY ? m_run : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = exp2f(fmaf(s[u >> 1][(u & 1) * 8 + i], f, -m_use));
+                    l += e;
+                    x[i] = e;
+                    if constexpr (NP == 2) x[i] *= pfac;
+                }
+                const uint4 hi = round8<E>(x);
+                uint4 lo;
+                if constexpr (NP == 2) lo = rest8(x);
+#pragma unroll
+                for (int t = 0; t < ND; ++t) {
+                    const uint4 vh = *(const uint4 *)(vl + (t * 4 + u) * 1024);
+                    o[t] = mfma<E>(vh, hi, o[t]);
+                    if constexpr (NP == 2) {
+                        const uint4 vlo = *(const uint4 *)(vl + PLANE + (t * 4 + u) * 1024);
+                        o[t] = mfma<E>(vh, lo, o[t]);
+                        o[t] = mfma<E>(vlo, hi, o[t]);
+                    }
+                }
+            }
+            if (odd) {
+                // values that are not finite, left out of the product: the
+                // rows that see their key take them as they are
+#pragma unroll 1
+                for (int j = 0; j < kTile && key0 + j < p.n; ++j) {
+                    const int key = key0 + j;
+                    const bool in = key <= token && (a.window <= 0 || key > token - a.window);
+                    const T *v = (const T *)a.v + (p.start + key) * a.v_stride + head * D + 4 * half;
+#pragma unroll
+                    for (int t = 0; t < ND; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float x = (float)v[32 * t + 8 * (i >> 2) + (i & 3)];
+                            if (in && !(fabsf(x) <= FLT_MAX)) o[t][i] += x;
+                        }
+                }
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the next tile is in LDS
+        __syncthreads();
+    }
+
+    l = halves_sum(l);
+    if (row < rows) {
+        float g = l != 0.0f ? 1.0f / l : 0.0f;
+        if constexpr (NP == 2) g = ldexpf(g, ev_ref - kTopExp - kPExp);
+        T *out = (T *)a.out + (p.start + token) * a.out_stride + (head * group + hq) * D + 4 * half;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                T y[4] __attribute__((aligned(16)));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = (T)(o[t][4 * b + i] * g);
+                if constexpr (sizeof(T) == 4)
+                    *(float4 *)(out + 32 * t + 8 * b) = *(const float4 *)y;
+                else
+                    *(uint2 *)(out + 32 * t + 8 * b) = *(const uint2 *)y;
+            }
+    }
+}
+
+template <typename T, int D> hipError_t prompt_launch(const PromptArgs &a, hipStream_t st) {
+    constexpr int lds = 2 * tile_bytes<T, D>();
+    auto *attn = k_prompt_attn<T, D>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void *)attn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    k_prompt_pack<T, D><<<dim3((unsigned)a.n_tiles, (unsigned)a.n_kv_heads), 256, 0, st>>>(a);
+    attn<<<(unsigned)(a.n_slots * a.n_kv_heads), 2 * kPromptRows, lds, st>>>(a);
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t prompt_dim(int head_dim, const PromptArgs &a, hipStream_t st) {
+    return head_dim == 64 ? prompt_launch<T, 64>(a, st) : prompt_launch<T, 128>(a, st);
+}
+
+}  // namespace
+
+hipError_t launch_prompt_attn(int dtype, int head_dim, const PromptArgs &a, hipStream_t st) {
+    if (dtype == VKV_DTYPE_F16) return prompt_dim<_Float16>(head_dim, a, st);
+    if (dtype == VKV_DTYPE_BF16) return prompt_dim<__bf16>(head_dim, a, st);
+    return prompt_dim<float>(head_dim, a, st);
+}
+
+}  // namespace vkv

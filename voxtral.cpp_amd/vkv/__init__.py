@@ -45,6 +45,9 @@ Q8_0 = 8
 Q4_K = 12
 Q6_K = 14
 Q8_K = 15
+I8 = 24
+BF16 = 30
+E4M3 = 100
 MAX_BATCH_STREAMS = 32
 KQ_BLOCK_BYTES = {Q4_K: 144, Q6_K: 210, Q8_K: 292, Q8_0: 272}   # bytes per 256 elements
 MV_MAX_IN = 12288
@@ -189,6 +192,13 @@ class Adapter(ctypes.Structure):
                 ("enc_dim", _i32), ("dec_dim", _i32), ("downsample", _i32)]
 
 
+class Pages(ctypes.Structure):
+    """A pool of 8-bit K/V pages in the caller's memory (vkv_pages)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("dtype", _i32),
+                ("n_layers", _i32), ("n_pages", _i32), ("page_size", _i32), ("n_kv_heads", _i32),
+                ("head_dim", _i32)]
+
+
 class GgufTensor(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("type", _i32), ("n_dims", _i32), ("ne", _i64 * 4),
                 ("offset", _u64), ("nbytes", _u64)]
@@ -306,6 +316,18 @@ PROTOTYPES = {
     "vkv_model_free": (_i32, [_vp]),
     "vkv_model_get_view": (_i32, [_vp, _P(ModelView)]),
     "vkv_model_tensor": (_vp, [_vp, ctypes.c_char_p, _P(GgufTensor)]),
+    "vkv_page_map": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp,
+                            _vp, _vp, _vp, _vp]),
+    "vkv_pages_append": (_i32, [_P(Pages), _i32, _vp, _i32, _i32, _vp, _vp, _i64, _vp]),
+    "vkv_paged_attn_workspace": (ctypes.c_size_t, [_P(Pages), _i32, _i32, _i32]),
+    "vkv_paged_attn": (_i32, [_P(Pages), _i32, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _i64,
+                              _vp, _i64, _i32, _f32, _vp, ctypes.c_size_t, _vp]),
+    "vkv_prompt_attn_workspace": (ctypes.c_size_t, [_i32] * 5),
+    "vkv_prompt_attn": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32,
+                               _i32, _f32, _i32, _vp, _i64, _vp, ctypes.c_size_t, _vp]),
+    "vkv_logprobs_workspace": (ctypes.c_size_t, [_i32, _i64, _i32]),
+    "vkv_logprobs": (_i32, [_i32, _vp, _i64, _i32, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp,
+                            ctypes.c_size_t, _vp]),
     "vkv_synth_rows": (_i32, [_vp, _i32, _u64, _u32, _i64, _i32, _i64, _i64, _i32, _i64, _i64,
                               _i32, _i64, _vp]),
     "vkv_api_version": (_u32, []),
@@ -834,3 +856,53 @@ class Model:
     def __del__(self):
         self.close()
 
+
+# many requests over one pool of 8-bit pages --------------------------------
+def page_map(len_old, len_new, n_req, page_size, n_pages, table, table_stride, free_pages, n_free,
+             n_free_out, max_tokens, len_out, cu_new, slots, positions, status, hip_stream=0):
+    """Block tables, slots and positions of a step from the requests' lengths (vkv_page_map)."""
+    check(lib.vkv_page_map(len_old, len_new, n_req, page_size, n_pages, table, table_stride,
+                           free_pages, n_free, n_free_out, max_tokens, len_out, cu_new, slots,
+                           positions, status, hip_stream))
+
+
+def pages_append(pages, layer, slots, n_tokens, dtype, k, v, row_stride=0, hip_stream=0):
+    """K and V rows into one layer's pages (vkv_pages_append)."""
+    check(lib.vkv_pages_append(ctypes.byref(pages), layer, slots, n_tokens, dtype, k, v, row_stride,
+                               hip_stream))
+
+
+def paged_attn_workspace(pages, n_rows, n_q_heads, max_len):
+    return int(lib.vkv_paged_attn_workspace(ctypes.byref(pages), n_rows, n_q_heads, max_len))
+
+
+def paged_attn(pages, layer, table, table_stride, lens, n_rows, max_len, dtype, q, out, n_q_heads,
+               scale, window=0, ws=0, ws_bytes=0, q_stride=0, out_stride=0, hip_stream=0):
+    """Single-query attention over one layer's pages (vkv_paged_attn)."""
+    check(lib.vkv_paged_attn(ctypes.byref(pages), layer, table, table_stride, lens, n_rows, max_len,
+                             window, dtype, q, q_stride, out, out_stride, n_q_heads, scale, ws,
+                             ws_bytes, hip_stream))
+
+
+def prompt_attn_workspace(dtype, n_seq, n_tokens, n_kv_heads, head_dim):
+    return int(lib.vkv_prompt_attn_workspace(dtype, n_seq, n_tokens, n_kv_heads, head_dim))
+
+
+def prompt_attn(dtype, q, k, v, cu_seqlens, n_seq, n_tokens, n_q_heads, n_kv_heads, head_dim, scale,
+                window, out, ws, ws_bytes, q_stride=0, k_stride=0, v_stride=0, out_stride=0,
+                hip_stream=0):
+    """Causal attention of packed prompts (vkv_prompt_attn)."""
+    check(lib.vkv_prompt_attn(dtype, q, q_stride, k, k_stride, v, v_stride, cu_seqlens, n_seq,
+                              n_tokens, n_q_heads, n_kv_heads, head_dim, scale, window, out,
+                              out_stride, ws, ws_bytes, hip_stream))
+
+
+def logprobs_workspace(n_rows, n_vocab, n_top):
+    return int(lib.vkv_logprobs_workspace(n_rows, n_vocab, n_top))
+
+
+def logprobs(dtype, logits, n_rows, n_vocab, tokens, logprob, entropy, n_top, top_ids, top_logprobs,
+             ws, ws_bytes, row_stride=0, hip_stream=0):
+    """Log probabilities of given tokens, entropy and likeliest tokens of rows (vkv_logprobs)."""
+    check(lib.vkv_logprobs(dtype, logits, row_stride, n_rows, n_vocab, tokens, logprob, entropy,
+                           n_top, top_ids, top_logprobs, ws, ws_bytes, hip_stream))
