@@ -62,13 +62,13 @@ template <typename E> __device__ __forceinline__ uint4 round8(const float *x) {
     return __builtin_bit_cast(uint4, r);
 }
 
-// and what that leaves of them; nothing of what is not finite
-__device__ __forceinline__ uint4 rest8(const float *x) {
+// and what that leaves of them; CHECK: nothing of what is not finite
+template <bool CHECK> __device__ __forceinline__ uint4 rest8(const float *x) {
     half8_t r;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float hi = (float)(_Float16)x[i];
-        r[i] = (_Float16)(fabsf(hi) <= FLT_MAX ? x[i] - hi : 0.0f);
+        r[i] = (_Float16)(!CHECK || fabsf(hi) <= FLT_MAX ? x[i] - hi : 0.0f);
     }
     return __builtin_bit_cast(uint4, r);
 }
@@ -112,7 +112,9 @@ struct Prompt {
 // least ceil(n_i * mul / per) of them lie before prompt i + 1's, so the place
 // of every slot follows from the offsets alone, without a sum over the
 // prompts.  Offsets are held to [0, n_tokens], whatever they are.
-__device__ __forceinline__ int offset_of(const PromptArgs &a, int i) { return min(max(a.cu[i], 0), a.n_tokens); }
+__device__ __forceinline__ int offset_of(const PromptArgs &a, int i) {
+    return min(max(((const __attribute__((address_space(4))) int32_t *)a.cu)[i], 0), a.n_tokens);
+}
 __device__ __forceinline__ bool find_prompt(const PromptArgs &a, int64_t slot, int mul, int per, Prompt &p) {
     const int lane = threadIdx.x & 63;
     int lo = 0, hi = a.n_seq;
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
         const int piece = tid + 256 * s;
         if constexpr (NP == 2) {
             for (int i = 0; i < 8; ++i) kx[s][i] = ldexpf(kx[s][i], kTopExp - ek);
-            out[PLANE + piece] = rest8(kx[s]);
+            out[PLANE + piece] = rest8<true>(kx[s]);
         }
         out[piece] = round8<E>(kx[s]);
         const int l = piece & 63, u = (piece >> 6) & 3, dt = piece >> 8;
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
             x[i] = vt[key][32 * dt + (l & 31)];
             if constexpr (NP == 2) x[i] = ldexpf(x[i], kTopExp - ev);
         }
-        if constexpr (NP == 2) out[3 * PLANE + piece] = rest8(x);
+        if constexpr (NP == 2) out[3 * PLANE + piece] = rest8<true>(x);
         out[NP * PLANE + piece] = round8<E>(x);
     }
     if (tid == 0) {
@@ -235,6 +237,140 @@ __global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
     }
 }
 
+// What a wave keeps of its 32 rows: their columns of Q, of O^T, the running
+// maximum (in log2 units) and sum of a column, each lane its own half of the
+// keys, and the exponent that O's weights were scaled by.
+template <typename T, int D> struct Rows {
+    uint4 q[Operand<T>::planes][D / 16];
+    floatx16 o[D / 32];
+    float factor, m, l;
+    int ev_ref;
+    int token, t_first, t_last;
+};
+
+// What k_prompt_pack says of a tile, read as the constants they are here.
+typedef int TileInfo __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ TileInfo tile_info(const PromptArgs &a, int64_t tile) {
+    return ((const __attribute__((address_space(4))) TileInfo *)a.info)[tile];
+}
+
+// One tile of keys.  `next` (unless null) is fetched into the other buffer on
+// the way: the two are restrict, or each read of this tile would wait for it.
+template <typename T, int D>
+__device__ __forceinline__ void tile_step(const PromptArgs &a, const Prompt &p, int head, TileInfo info, int kt,
+                                          const uint8_t *__restrict__ cur, uint8_t *__restrict__ other,
+                                          const uint8_t *next, bool seen, Rows<T, D> &r) {
+    typedef typename Operand<T>::elem E;
+    constexpr int NP = Operand<T>::planes, NM = D / 16, ND = D / 32;
+    constexpr int BYTES = tile_bytes<T, D>(), PLANE = kTile * D * 2;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    if (next) {
+#pragma unroll
+        for (int i = 0; i < BYTES / (2 * kPromptRows * 16); ++i)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) unsigned *)(next + threadIdx.x * 16 + i * (2 * kPromptRows * 16)),
+                (__attribute__((address_space(3))) unsigned *)(other + i * (2 * kPromptRows * 16) + (threadIdx.x & ~63) * 16),
+                16, 0, 0);
+    }
+    if (!seen) return;
+    const int key0 = kt * kTile;
+    const uint8_t *kl = cur + lane * 16, *vl = kl + NP * PLANE;
+    const int ek = info[0], ev = info[1], odd = info[2];
+    const float f = fmaxf(NP == 2 ? ldexpf(r.factor, ek - kTopExp) : r.factor, FLT_MIN);
+    floatx16 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            const uint4 hi = *(const uint4 *)(kl + (kb * NM + m) * 1024);
+            s[kb] = mfma<E>(hi, r.q[0][m], s[kb]);
+            if constexpr (NP == 2) {
+                const uint4 lo = *(const uint4 *)(kl + PLANE + (kb * NM + m) * 1024);
+                s[kb] = mfma<E>(hi, r.q[1][m], s[kb]);
+                s[kb] = mfma<E>(lo, r.q[0][m], s[kb]);
+            }
+        }
+    }
+    if (key0 + kTile - 1 > r.t_first || (a.window > 0 && key0 <= r.t_last - a.window)) {
+        // keys [low, high] of the tile, counted from this lane's first
+        const int first = key0 + 4 * half;
+        const int high = r.token - first, low = a.window > 0 ? high - a.window + 1 : INT32_MIN;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = 32 * kb + 8 * (i >> 2) + (i & 3);
+                s[kb][i] = j <= high && j >= low ? s[kb][i] : -INFINITY;
+            }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
+    mx = halves_max(mx) * f;
+    // the running maximum moves only when it is passed by 2^8
+    if (__any(mx > r.m + 8.0f)) {
+        const float m_new = fmaxf(r.m, mx);
+        const float g = m_new > -INFINITY ? __builtin_amdgcn_exp2f(r.m - m_new) : 1.0f;
+        r.l *= g;
+#pragma unroll
+        for (int t = 0; t < ND; ++t) r.o[t] *= g;
+        r.m = m_new;
+    }
+    float pfac = 1.0f;
+    if constexpr (NP == 2) {
+        if (ev > r.ev_ref) {
+            const float g = ldexpf(1.0f, max(r.ev_ref - ev, -300));
+#pragma unroll
+            for (int t = 0; t < ND; ++t) r.o[t] *= g;
+            r.ev_ref = ev;
+        }
+        pfac = ldexpf(1.0f, kPExp + ev - r.ev_ref);
+    }
+    const float m_use = r.m > -INFINITY ? -r.m : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][(u & 1) * 8 + i], f, m_use));
+            r.l += e;
+            x[i] = NP == 2 ? e * pfac : e;
+        }
+        const uint4 hi = round8<E>(x);
+        uint4 lo;
+        if constexpr (NP == 2) lo = rest8<false>(x);
+#pragma unroll
+        for (int t = 0; t < ND; ++t) {
+            const uint4 vh = *(const uint4 *)(vl + (t * 4 + u) * 1024);
+            r.o[t] = mfma<E>(vh, hi, r.o[t]);
+            if constexpr (NP == 2) {
+                const uint4 vlo = *(const uint4 *)(vl + PLANE + (t * 4 + u) * 1024);
+                r.o[t] = mfma<E>(vh, lo, r.o[t]);
+                r.o[t] = mfma<E>(vlo, hi, r.o[t]);
+            }
+        }
+    }
+    if (odd) {
+        // values that are not finite, left out of the product: the rows that
+        // see their key take them as they are
+#pragma unroll 1
+        for (int j = 0; j < kTile && key0 + j < p.n; ++j) {
+            const int key = key0 + j;
+            const bool in = key <= r.token && (a.window <= 0 || key > r.token - a.window);
+            const T *v = (const T *)a.v + (p.start + key) * a.v_stride + head * D + 4 * half;
+#pragma unroll
+            for (int t = 0; t < ND; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = (float)v[32 * t + 8 * (i >> 2) + (i & 3)];
+                    if (in && !(fabsf(x) <= FLT_MAX)) r.o[t][i] += x;
+                }
+        }
+    }
+}
+
 // A work group: 8 waves on 256 rows of one (prompt, kv head), a row being
 // (token, query head of the kv head), so the heads that share K and V read one
 // copy of them in LDS.  Wave w owns rows 32 w + [0, 32) as the columns of S^T =
@@ -242,12 +378,11 @@ __global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
 // second product, so P stays in its registers.  Key tiles are double-buffered
 // in LDS by loads that go there without registers.
 template <typename T, int D>
-__global__ __launch_bounds__(2 * kPromptRows) void k_prompt_attn(PromptArgs a) {
+__global__ __launch_bounds__(2 * kPromptRows) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_prompt_attn(PromptArgs a) {
     typedef typename Operand<T>::elem E;
     constexpr int NP = Operand<T>::planes;
     constexpr int NM = D / 16, ND = D / 32;
     constexpr int BYTES = tile_bytes<T, D>();
-    constexpr int PLANE = kTile * D * 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -259,39 +394,31 @@ __global__ __launch_bounds__(2 * kPromptRows) void k_prompt_attn(PromptArgs a) {
     const int64_t slot = a.n_slots - 1 - blockIdx.x / a.n_kv_heads;
     Prompt p;
     if (!find_prompt(a, slot, group, kPromptRows, p)) return;
-    const int64_t rows = (int64_t)p.n * group;
-    const int64_t row0 = (int64_t)p.local * kPromptRows;
+    // a call's rows are fewer than 2^31
+    const unsigned rows = (unsigned)p.n * (unsigned)group;
+    const unsigned row0 = (unsigned)p.local * kPromptRows;
     if (row0 >= rows) return;
 
-    const int64_t wrow = row0 + 32 * wave;
+    const unsigned wrow = row0 + 32 * wave;
     const bool busy = wrow < rows;
-    const int64_t row = wrow + (lane & 31);
-    const int64_t row_in = row < rows ? row : rows - 1;
-    const int token = (int)(row_in / group), hq = (int)(row_in % group);
-    const int t_first = (int)((busy ? wrow : rows - 1) / group);
-    const int t_last = (int)((wrow + 31 < rows ? wrow + 31 : rows - 1) / group);
-    const int wg_first = (int)(row0 / group);
-    const int wg_last = (int)((row0 + kPromptRows - 1 < rows ? row0 + kPromptRows - 1 : rows - 1) / group);
+    const unsigned row = wrow + (lane & 31), row_in = min(row, rows - 1);
+    Rows<T, D> r;
+    r.token = (int)(row_in / (unsigned)group);
+    const int hq = (int)(row_in - (unsigned)r.token * (unsigned)group);
+    r.t_first = __builtin_amdgcn_readlane(r.token, 0);
+    r.t_last = __builtin_amdgcn_readlane(r.token, 31);
+    const int wg_first = (int)(row0 / (unsigned)group);
+    const int wg_last = (int)(min(row0 + kPromptRows, rows) - 1) / group;
     const int kt0 = a.window > 0 && wg_first >= a.window ? (wg_first - a.window + 1) / kTile : 0;
     const int kt1 = wg_last / kTile;
     const int64_t tile0 = (int64_t)head * a.n_tiles + p.start / kTile + p.seq;
-
-    auto fetch = [&](int kt, int buf) {
-        const uint8_t *src = a.data + (tile0 + kt) * BYTES + tid * 16;
-#pragma unroll
-        for (int i = 0; i < BYTES / (2 * kPromptRows * 16); ++i)
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) unsigned *)(src + i * (2 * kPromptRows * 16)),
-                (__attribute__((address_space(3))) unsigned *)(lds + buf * BYTES + i * (2 * kPromptRows * 16) + wave * 1024),
-                16, 0, 0);
-    };
-    fetch(kt0, 0);
+    TileInfo info = tile_info(a, tile0 + kt0);
+    tile_step<T, D>(a, p, head, info, 0, lds + BYTES, lds, a.data + (tile0 + kt0) * BYTES, false, r);
 
     // this lane's column of Q: dims 16 m + 8 half + [0, 8)
-    uint4 qf[NP][NM];
-    float qfac = fabsf(a.scale) * kLog2e;
+    r.factor = fabsf(a.scale) * kLog2e;
     {
-        const T *q = (const T *)a.q + (p.start + token) * a.q_stride + (head * group + hq) * D + 8 * half;
+        const T *q = (const T *)a.q + (p.start + r.token) * a.q_stride + (head * group + hq) * D + 8 * half;
         float x[NM][8];
         float qmax = 0.0f;
 #pragma unroll
@@ -299,152 +426,57 @@ __global__ __launch_bounds__(2 * kPromptRows) void k_prompt_attn(PromptArgs a) {
             load8(q + 16 * m, x[m]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
+                if (NP == 2) qmax = fmaxf(qmax, finite_abs(x[m][i]));
                 if (a.scale < 0.0f) x[m][i] = -x[m][i];
-                qmax = fmaxf(qmax, finite_abs(x[m][i]));
             }
         }
         if constexpr (NP == 2) {
             const int e = exponent(halves_max(qmax));
-            qfac = ldexpf(qfac, e - kTopExp);
+            r.factor = ldexpf(r.factor, e - kTopExp);
 #pragma unroll
             for (int m = 0; m < NM; ++m) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[m][i] = ldexpf(x[m][i], kTopExp - e);
-                qf[1][m] = rest8(x[m]);
+                r.q[1][m] = rest8<true>(x[m]);
             }
         }
 #pragma unroll
-        for (int m = 0; m < NM; ++m) qf[0][m] = round8<E>(x[m]);
+        for (int m = 0; m < NM; ++m) r.q[0][m] = round8<E>(x[m]);
     }
-
-    floatx16 o[ND];
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-    float m_run = -INFINITY, l = 0.0f;
-    int ev_ref = -1000;
+        for (int i = 0; i < 16; ++i) r.o[t][i] = 0.0f;
+    r.m = -INFINITY;
+    r.l = 0.0f;
+    r.ev_ref = -1000;
 
     __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
     __syncthreads();
     for (int kt = kt0; kt <= kt1; ++kt) {
         const int buf = (kt - kt0) & 1;
-        if (kt < kt1) fetch(kt + 1, buf ^ 1);
         const int key0 = kt * kTile;
-        const bool seen = busy && key0 <= t_last && (a.window <= 0 || key0 + kTile > t_first - a.window + 1);
-        if (seen) {
-            const uint8_t *kl = lds + buf * BYTES + lane * 16, *vl = kl + NP * PLANE;
-            const int32_t *info = a.info + (tile0 + kt) * 4;
-            const int ek = info[0], ev = info[1], odd = info[2];
-            const float f = fmaxf(NP == 2 ? ldexpf(qfac, ek - kTopExp) : qfac, FLT_MIN);
-            floatx16 s[2];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
-#pragma unroll
-                for (int m = 0; m < NM; ++m) {
-                    const uint4 hi = *(const uint4 *)(kl + (kb * NM + m) * 1024);
-                    s[kb] = mfma<E>(hi, qf[0][m], s[kb]);
-                    if constexpr (NP == 2) {
-                        const uint4 lo = *(const uint4 *)(kl + PLANE + (kb * NM + m) * 1024);
-                        s[kb] = mfma<E>(hi, qf[1][m], s[kb]);
-                        s[kb] = mfma<E>(lo, qf[0][m], s[kb]);
-                    }
-                }
-            }
-            if (key0 + kTile - 1 > t_first || (a.window > 0 && key0 <= t_last - a.window)) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = key0 + 32 * kb + 8 * (i >> 2) + 4 * half + (i & 3);
-                        const bool in = key <= token && (a.window <= 0 || key > token - a.window);
-                        s[kb][i] = in ? s[kb][i] : -INFINITY;
-                    }
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
-            mx = halves_max(mx) * f;
-            // the running maximum moves only when it is passed by 2^8
-            if (__any(mx > m_run + 8.0f)) {
-                const float m_new = fmaxf(m_run, mx);
-                const float g = m_new > -INFINITY ? exp2f(m_run - m_new) : 1.0f;
-                l *= g;
-#pragma unroll
-                for (int t = 0; t < ND; ++t) o[t] *= g;
-                m_run = m_new;
-            }
-            float pfac = 1.0f;
-            if constexpr (NP == 2) {
-                if (ev > ev_ref) {
-                    const float g = ldexpf(1.0f, max(ev_ref - ev, -300));
-#pragma unroll
-                    for (int t = 0; t < ND; ++t) o[t] *= g;
-                    ev_ref = ev;
-                }
-                pfac = ldexpf(1.0f, kPExp + ev - ev_ref);
-            }
-            const float m_use = m_run > -INFINITY ? m_run : 0.0f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float e = exp2f(fmaf(s[u >> 1][(u & 1) * 8 + i], f, -m_use));
-                    l += e;
-                    x[i] = e;
-                    if constexpr (NP == 2) x[i] *= pfac;
-                }
-                const uint4 hi = round8<E>(x);
-                uint4 lo;
-                if constexpr (NP == 2) lo = rest8(x);
-#pragma unroll
-                for (int t = 0; t < ND; ++t) {
-                    const uint4 vh = *(const uint4 *)(vl + (t * 4 + u) * 1024);
-                    o[t] = mfma<E>(vh, hi, o[t]);
-                    if constexpr (NP == 2) {
-                        const uint4 vlo = *(const uint4 *)(vl + PLANE + (t * 4 + u) * 1024);
-                        o[t] = mfma<E>(vh, lo, o[t]);
-                        o[t] = mfma<E>(vlo, hi, o[t]);
-                    }
-                }
-            }
-            if (odd) {
-                // values that are not finite, left out of the product: the
-                // rows that see their key take them as they are
-#pragma unroll 1
-                for (int j = 0; j < kTile && key0 + j < p.n; ++j) {
-                    const int key = key0 + j;
-                    const bool in = key <= token && (a.window <= 0 || key > token - a.window);
-                    const T *v = (const T *)a.v + (p.start + key) * a.v_stride + head * D + 4 * half;
-#pragma unroll
-                    for (int t = 0; t < ND; ++t)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float x = (float)v[32 * t + 8 * (i >> 2) + (i & 3)];
-                            if (in && !(fabsf(x) <= FLT_MAX)) o[t][i] += x;
-                        }
-                }
-            }
-        }
+        const bool seen = busy && key0 <= r.t_last && (a.window <= 0 || key0 + kTile > r.t_first - a.window + 1);
+        const TileInfo next_info = tile_info(a, tile0 + min(kt + 1, kt1));
+        tile_step<T, D>(a, p, head, info, kt, lds + buf * BYTES, lds + (buf ^ 1) * BYTES,
+                        kt < kt1 ? a.data + (tile0 + kt + 1) * BYTES : nullptr, seen, r);
+        info = next_info;
         __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the next tile is in LDS
         __syncthreads();
     }
 
-    l = halves_sum(l);
+    const float l = halves_sum(r.l);
     if (row < rows) {
         float g = l != 0.0f ? 1.0f / l : 0.0f;
-        if constexpr (NP == 2) g = ldexpf(g, ev_ref - kTopExp - kPExp);
-        T *out = (T *)a.out + (p.start + token) * a.out_stride + (head * group + hq) * D + 4 * half;
+        if constexpr (NP == 2) g = ldexpf(g, r.ev_ref - kTopExp - kPExp);
+        T *out = (T *)a.out + (p.start + r.token) * a.out_stride + (head * group + hq) * D + 4 * half;
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 T y[4] __attribute__((aligned(16)));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = (T)(o[t][4 * b + i] * g);
+                for (int i = 0; i < 4; ++i) y[i] = (T)(r.o[t][4 * b + i] * g);
                 if constexpr (sizeof(T) == 4)
                     *(float4 *)(out + 32 * t + 8 * b) = *(const float4 *)y;
                 else
