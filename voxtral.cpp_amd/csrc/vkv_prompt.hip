@@ -135,6 +135,15 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs &a, int64_t slot, i
     return true;
 }
 
+// What k_prompt_pack says of a tile: the exponents of K and V and whether V
+// holds what is not finite, in one word.
+struct TileInfo {
+    int word;
+    __device__ int ek() const { return (word & 1023) - 512; }
+    __device__ int ev() const { return (word >> 10 & 1023) - 512; }
+    __device__ int odd() const { return word >> 20; }
+};
+
 // A tile's operands: K, planes x [2 blocks of 32 keys][D/16][64 lanes] 16
 // bytes: lane (r, h) has key 32 kb + r, dims 16 m + 8 h + [0, 8).  V, planes x
 // [D/32][4 blocks of 16 keys][64 lanes]: lane (r, h) has dim 32 dt + r, keys
@@ -228,86 +237,153 @@ __global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
         if constexpr (NP == 2) out[3 * PLANE + piece] = rest8<true>(x);
         out[NP * PLANE + piece] = round8<E>(x);
     }
-    if (tid == 0) {
-        int32_t *info = a.info + tile * 4;
-        info[0] = ek;
-        info[1] = ev;
-        info[2] = odd;
-        info[3] = 0;
-    }
+    if (tid == 0) a.info[tile] = (ek + 512) | (ev + 512) << 10 | odd << 20;
 }
 
-// What a wave keeps of its 32 rows: their columns of Q, of O^T, the running
-// maximum (in log2 units) and sum of a column, each lane its own half of the
-// keys, and the exponent that O's weights were scaled by.
+constexpr int kPromptThreads = 2 * kPromptRows;
+
+constexpr int kLoadThreads = kPromptThreads / 2;    // the first four waves fetch
+
+// Half a tile (K or V) into LDS without registers; buffer loads, beside which
+// the waits for LDS reads stay counted.
+template <int BYTES> __device__ __forceinline__ void fetch(const uint8_t *src, uint8_t *dst, int wave) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)src, 0, BYTES, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < BYTES / (kLoadThreads * 16); ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rsrc, (__attribute__((address_space(3))) void *)(dst + i * (kLoadThreads * 16) + wave * 1024), 16,
+            threadIdx.x * 16, i * (kLoadThreads * 16), 0, 0);
+}
+
+__device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
+
+// none of the wave's LDS reads are under way, and the others are as far
+__device__ __forceinline__ void meet() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+}
+
+// A wave's 32 rows: their columns of Q and of O^T; the scores of a tile, then
+// its weights; the running maximum (in log2 units) and the sum of each column,
+// every lane its own half of the keys; the factor of the scores; the exponent
+// that O's weights are scaled by.
 template <typename T, int D> struct Rows {
-    uint4 q[Operand<T>::planes][D / 16];
-    floatx16 o[D / 32];
+    uint4 q[Operand<T>::planes][D / 16], p[Operand<T>::planes][4];
+    floatx16 o[D / 32], s[2];
     float factor, m, l;
     int ev_ref;
     int token, t_first, t_last;
+    int first_tile, last_tile;      // of those the wave sees
 };
 
-// What k_prompt_pack says of a tile, read as the constants they are here.
-typedef int TileInfo __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ TileInfo tile_info(const PromptArgs &a, int64_t tile) {
-    return ((const __attribute__((address_space(4))) TileInfo *)a.info)[tile];
-}
-
-// One tile of keys.  `next` (unless null) is fetched into the other buffer on
-// the way: the two are restrict, or each read of this tile would wait for it.
-template <typename T, int D>
-__device__ __forceinline__ void tile_step(const PromptArgs &a, const Prompt &p, int head, TileInfo info, int kt,
-                                          const uint8_t *__restrict__ cur, uint8_t *__restrict__ other,
-                                          const uint8_t *next, bool seen, Rows<T, D> &r) {
+// S^T of the tile whose K is at k
+template <typename T, int D> __device__ __forceinline__ void scores(Rows<T, D> &r, const uint8_t *k) {
     typedef typename Operand<T>::elem E;
-    constexpr int NP = Operand<T>::planes, NM = D / 16, ND = D / 32;
-    constexpr int BYTES = tile_bytes<T, D>(), PLANE = kTile * D * 2;
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    if (next) {
+    constexpr int NP = Operand<T>::planes, NM = D / 16, PLANE = kTile * D * 2;
+    k += (threadIdx.x & 63) * 16;
 #pragma unroll
-        for (int i = 0; i < BYTES / (2 * kPromptRows * 16); ++i)
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) unsigned *)(next + threadIdx.x * 16 + i * (2 * kPromptRows * 16)),
-                (__attribute__((address_space(3))) unsigned *)(other + i * (2 * kPromptRows * 16) + (threadIdx.x & ~63) * 16),
-                16, 0, 0);
-    }
-    if (!seen) return;
-    const int key0 = kt * kTile;
-    const uint8_t *kl = cur + lane * 16, *vl = kl + NP * PLANE;
-    const int ek = info[0], ev = info[1], odd = info[2];
-    const float f = fmaxf(NP == 2 ? ldexpf(r.factor, ek - kTopExp) : r.factor, FLT_MIN);
-    floatx16 s[2];
+    for (int i = 0; i < 32; ++i) r.s[i >> 4][i & 15] = 0.0f;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int m = 0; m < NM; ++m)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            const uint4 hi = *(const uint4 *)(kl + (kb * NM + m) * 1024);
-            s[kb] = mfma<E>(hi, r.q[0][m], s[kb]);
+        for (int kb = 0; kb < 2; ++kb) {
+            const uint4 hi = *(const uint4 *)(k + (kb * NM + m) * 1024);
+            r.s[kb] = mfma<E>(hi, r.q[0][m], r.s[kb]);
             if constexpr (NP == 2) {
-                const uint4 lo = *(const uint4 *)(kl + PLANE + (kb * NM + m) * 1024);
-                s[kb] = mfma<E>(hi, r.q[1][m], s[kb]);
-                s[kb] = mfma<E>(lo, r.q[0][m], s[kb]);
+                const uint4 lo = *(const uint4 *)(k + PLANE + (kb * NM + m) * 1024);
+                r.s[kb] = mfma<E>(hi, r.q[1][m], r.s[kb]);
+                r.s[kb] = mfma<E>(lo, r.q[0][m], r.s[kb]);
             }
         }
+}
+
+// The matrix cores' half of a tile: O^T += V^T P^T for the tile whose weights
+// are at hand, and the scores of the next.  The next tile's operands are
+// fetched into the other places on the way: the four are restrict, or each
+// read would wait for the loads.
+template <typename T, int D>
+__device__ __forceinline__ void products(const PromptArgs &a, const Prompt &p, int head, int kt, int odd, bool fetches, int wave,
+                                         const uint8_t *k_src, const uint8_t *v_src, const uint8_t *__restrict__ k_cur,
+                                         uint8_t *__restrict__ k_next, const uint8_t *__restrict__ v_cur,
+                                         uint8_t *__restrict__ v_next, Rows<T, D> &r) {
+    typedef typename Operand<T>::elem E;
+    constexpr int NP = Operand<T>::planes, NM = D / 16, ND = D / 32;
+    constexpr int HALF = tile_bytes<T, D>() / 2, PLANE = kTile * D * 2;
+    const int lane = threadIdx.x & 63;
+    if (fetches) {
+        fetch<HALF>(k_src, k_next, wave);
+        fetch<HALF>(v_src, v_next, wave);
     }
-    if (key0 + kTile - 1 > r.t_first || (a.window > 0 && key0 <= r.t_last - a.window)) {
-        // keys [low, high] of the tile, counted from this lane's first
-        const int first = key0 + 4 * half;
-        const int high = r.token - first, low = a.window > 0 ? high - a.window + 1 : INT32_MIN;
+    if (kt + 1 < r.first_tile || kt > r.last_tile) return;
+    __builtin_amdgcn_s_setprio(1);
+    const uint8_t *v = v_cur + lane * 16;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int j = 32 * kb + 8 * (i >> 2) + (i & 3);
-                s[kb][i] = j <= high && j >= low ? s[kb][i] : -INFINITY;
+        for (int t = 0; t < ND; ++t) {
+            const uint4 vh = *(const uint4 *)(v + (t * 4 + u) * 1024);
+            r.o[t] = mfma<E>(vh, r.p[0][u], r.o[t]);
+            if constexpr (NP == 2) {
+                r.o[t] = mfma<E>(vh, r.p[1][u], r.o[t]);
+                r.o[t] = mfma<E>(*(const uint4 *)(v + PLANE + (t * 4 + u) * 1024), r.p[0][u], r.o[t]);
             }
-    }
-    float mx = s[0][0];
+        }
+    scores(r, k_cur);
+    // a few operands are read ahead of the products
+    constexpr int AHEAD = NP == 2 ? 2 : 6, PAIRS = 4 * ND + 2 * NM;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * NP, 0);
 #pragma unroll
-    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i >> 4][i & 15]);
+    for (int i = 0; i < PAIRS - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NP == 2 ? 3 : 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (odd) {
+        // values that are not finite, left out of the product: the rows that
+        // see their key take them as they are
+#pragma unroll 1
+        for (int key = kt * kTile; key < (kt + 1) * kTile && key < p.n; ++key) {
+            const bool in = key <= r.token && (a.window <= 0 || key > r.token - a.window);
+            const T *x = (const T *)a.v + (p.start + key) * a.v_stride + head * D + 4 * (lane >> 5);
+#pragma unroll
+            for (int t = 0; t < ND; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float y = (float)x[32 * t + 8 * (i >> 2) + (i & 3)];
+                    if (in && !(fabsf(y) <= FLT_MAX)) r.o[t][i] += y;
+                }
+        }
+    }
+}
+
+// The vector units' half: the scores of tile kt become weights, and the sums
+// so far are brought to the new maximum.
+template <typename T, int D>
+__device__ __forceinline__ void weights(const PromptArgs &a, int kt, TileInfo info, Rows<T, D> &r) {
+    typedef typename Operand<T>::elem E;
+    constexpr int NP = Operand<T>::planes, ND = D / 32;
+    if (kt < r.first_tile || kt > r.last_tile) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) r.p[n][u] = uint4{0, 0, 0, 0};
+        return;
+    }
+    const float f = fmaxf(NP == 2 ? ldexpf(r.factor, info.ek() - kTopExp) : r.factor, FLT_MIN);
+    const int key0 = kt * kTile;
+    if (key0 + kTile - 1 > r.t_first || (a.window > 0 && key0 <= r.t_last - a.window)) {
+        // keys [low, high], counted from this lane's first
+        const int high = r.token - key0 - 4 * (int)((threadIdx.x & 63) >> 5);
+        const int low = a.window > 0 ? high - a.window + 1 : INT32_MIN;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int j = 32 * (i >> 4) + 8 * (i >> 2 & 3) + (i & 3);
+            r.s[i >> 4][i & 15] = j <= high && j >= low ? r.s[i >> 4][i & 15] : -INFINITY;
+        }
+    }
+    float mx = r.s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, r.s[i >> 4][i & 15]);
     mx = halves_max(mx) * f;
     // the running maximum moves only when it is passed by 2^8
     if (__any(mx > r.m + 8.0f)) {
@@ -320,6 +396,7 @@ __device__ __forceinline__ void tile_step(const PromptArgs &a, const Prompt &p, 
     }
     float pfac = 1.0f;
     if constexpr (NP == 2) {
+        const int ev = info.ev();
         if (ev > r.ev_ref) {
             const float g = ldexpf(1.0f, max(r.ev_ref - ev, -300));
 #pragma unroll
@@ -334,40 +411,12 @@ __device__ __forceinline__ void tile_step(const PromptArgs &a, const Prompt &p, 
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][(u & 1) * 8 + i], f, m_use));
+            const float e = __builtin_amdgcn_exp2f(fmaf(r.s[u >> 1][(u & 1) * 8 + i], f, m_use));
             r.l += e;
             x[i] = NP == 2 ? e * pfac : e;
         }
-        const uint4 hi = round8<E>(x);
-        uint4 lo;
-        if constexpr (NP == 2) lo = rest8<false>(x);
-#pragma unroll
-        for (int t = 0; t < ND; ++t) {
-            const uint4 vh = *(const uint4 *)(vl + (t * 4 + u) * 1024);
-            r.o[t] = mfma<E>(vh, hi, r.o[t]);
-            if constexpr (NP == 2) {
-                const uint4 vlo = *(const uint4 *)(vl + PLANE + (t * 4 + u) * 1024);
-                r.o[t] = mfma<E>(vh, lo, r.o[t]);
-                r.o[t] = mfma<E>(vlo, hi, r.o[t]);
-            }
-        }
-    }
-    if (odd) {
-        // values that are not finite, left out of the product: the rows that
-        // see their key take them as they are
-#pragma unroll 1
-        for (int j = 0; j < kTile && key0 + j < p.n; ++j) {
-            const int key = key0 + j;
-            const bool in = key <= r.token && (a.window <= 0 || key > r.token - a.window);
-            const T *v = (const T *)a.v + (p.start + key) * a.v_stride + head * D + 4 * half;
-#pragma unroll
-            for (int t = 0; t < ND; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float x = (float)v[32 * t + 8 * (i >> 2) + (i & 3)];
-                    if (in && !(fabsf(x) <= FLT_MAX)) r.o[t][i] += x;
-                }
-        }
+        r.p[0][u] = round8<E>(x);
+        if constexpr (NP == 2) r.p[1][u] = rest8<false>(x);
     }
 }
 
@@ -375,15 +424,22 @@ __device__ __forceinline__ void tile_step(const PromptArgs &a, const Prompt &p, 
 // (token, query head of the kv head), so the heads that share K and V read one
 // copy of them in LDS.  Wave w owns rows 32 w + [0, 32) as the columns of S^T =
 // K Q^T and O^T = V^T P^T; a lane's scores are the keys it supplies to the
-// second product, so P stays in its registers.  Key tiles are double-buffered
-// in LDS by loads that go there without registers.
+// second product, so P stays in its registers.
+//
+// The products of a tile and the softmax of a tile take about as long, on
+// units that can work at the same time, but waves that meet at every tile do
+// them at the same time and the units take turns.  So the second four waves
+// (one of the two on each SIMD) run half a tile behind the first: while one
+// wave of a SIMD multiplies, the other exponentiates.  Operands of tile kt's
+// turn (its V, the K of tile kt + 1) are in LDS for both halves of the turn;
+// those of the next come in meanwhile, by the first four waves.
 template <typename T, int D>
-__global__ __launch_bounds__(2 * kPromptRows) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_prompt_attn(PromptArgs a) {
+__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_prompt_attn(PromptArgs a) {
     typedef typename Operand<T>::elem E;
     constexpr int NP = Operand<T>::planes;
     constexpr int NM = D / 16, ND = D / 32;
-    constexpr int BYTES = tile_bytes<T, D>();
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr int BYTES = tile_bytes<T, D>(), HALF = BYTES / 2;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // K, K, V, V
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -399,21 +455,32 @@ __global__ __launch_bounds__(2 * kPromptRows) __attribute__((amdgpu_waves_per_eu
     const unsigned row0 = (unsigned)p.local * kPromptRows;
     if (row0 >= rows) return;
 
+    const bool ahead = wave < 4;
     const unsigned wrow = row0 + 32 * wave;
-    const bool busy = wrow < rows;
     const unsigned row = wrow + (lane & 31), row_in = min(row, rows - 1);
     Rows<T, D> r;
     r.token = (int)(row_in / (unsigned)group);
     const int hq = (int)(row_in - (unsigned)r.token * (unsigned)group);
     r.t_first = __builtin_amdgcn_readlane(r.token, 0);
     r.t_last = __builtin_amdgcn_readlane(r.token, 31);
+    r.first_tile = a.window > 0 && r.t_first >= a.window ? (r.t_first - a.window + 1) / kTile : 0;
+    r.last_tile = wrow < rows ? r.t_last / kTile : -2;      // a wave without rows sees no key
     const int wg_first = (int)(row0 / (unsigned)group);
     const int wg_last = (int)(min(row0 + kPromptRows, rows) - 1) / group;
     const int kt0 = a.window > 0 && wg_first >= a.window ? (wg_first - a.window + 1) / kTile : 0;
     const int kt1 = wg_last / kTile;
     const int64_t tile0 = (int64_t)head * a.n_tiles + p.start / kTile + p.seq;
-    TileInfo info = tile_info(a, tile0 + kt0);
-    tile_step<T, D>(a, p, head, info, 0, lds + BYTES, lds, a.data + (tile0 + kt0) * BYTES, false, r);
+    const uint8_t *data = a.data + tile0 * BYTES;
+    if (ahead) {
+        // K of the first tile where the turn before the first has it, then the first turn's operands
+        fetch<HALF>(data + (int64_t)kt0 * BYTES, lds + HALF, wave);
+        fetch<HALF>(data + (int64_t)min(kt0 + 1, kt1) * BYTES, lds, wave);
+        fetch<HALF>(data + (int64_t)kt0 * BYTES + HALF, lds + 2 * HALF, wave);
+    }
+    // the words of 64 tiles, a lane each: a load for every tile would have the
+    // waits for it cover the operands that are on their way
+    auto tile_words = [&](int kt) { return a.info[tile0 + min(kt + lane, kt1)]; };
+    int words = tile_words(kt0);
 
     // this lane's column of Q: dims 16 m + 8 half + [0, 8)
     r.factor = fabsf(a.scale) * kLog2e;
@@ -451,19 +518,33 @@ __global__ __launch_bounds__(2 * kPromptRows) __attribute__((amdgpu_waves_per_eu
     r.l = 0.0f;
     r.ev_ref = -1000;
 
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-    __syncthreads();
+    wait_for_memory();
+    meet();
+    if (!ahead) meet();
+    scores(r, lds + HALF);
+    meet();
+    TileInfo info{__builtin_amdgcn_readlane(words, 0)};
+    weights(a, kt0, info, r);
+    meet();
     for (int kt = kt0; kt <= kt1; ++kt) {
-        const int buf = (kt - kt0) & 1;
-        const int key0 = kt * kTile;
-        const bool seen = busy && key0 <= r.t_last && (a.window <= 0 || key0 + kTile > r.t_first - a.window + 1);
-        const TileInfo next_info = tile_info(a, tile0 + min(kt + 1, kt1));
-        tile_step<T, D>(a, p, head, info, kt, lds + buf * BYTES, lds + (buf ^ 1) * BYTES,
-                        kt < kt1 ? a.data + (tile0 + kt + 1) * BYTES : nullptr, seen, r);
-        info = next_info;
-        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the next tile is in LDS
-        __syncthreads();
+        const int cur = ((kt - kt0) & 1) * HALF, next = HALF - cur;
+        products<T, D>(a, p, head, kt, info.odd(), ahead && kt < kt1, wave,
+                       data + (int64_t)min(kt + 2, kt1) * BYTES,
+                       data + (int64_t)(kt + 1) * BYTES + HALF, lds + cur, lds + next, lds + 2 * HALF + cur,
+                       lds + 2 * HALF + next, r);
+        meet();
+        if (kt < kt1) {
+            if (((kt + 1 - kt0) & 63) == 0) {
+                words = tile_words(kt + 1);
+                asm volatile("" : "+v"(words));     // waited for here, not at every tile
+            }
+            info.word = __builtin_amdgcn_readlane(words, (kt + 1 - kt0) & 63);
+            weights(a, kt + 1, info, r);
+        }
+        if (ahead) wait_for_memory();
+        meet();
     }
+    if (ahead) meet();
 
     const float l = halves_sum(r.l);
     if (row < rows) {
@@ -493,7 +574,7 @@ template <typename T, int D> hipError_t prompt_launch(const PromptArgs &a, hipSt
         if (e != hipSuccess) return e;
     }
     k_prompt_pack<T, D><<<dim3((unsigned)a.n_tiles, (unsigned)a.n_kv_heads), 256, 0, st>>>(a);
-    attn<<<(unsigned)(a.n_slots * a.n_kv_heads), 2 * kPromptRows, lds, st>>>(a);
+    attn<<<(unsigned)(a.n_slots * a.n_kv_heads), kPromptThreads, lds, st>>>(a);
     return hipGetLastError();
 }
 

@@ -140,7 +140,7 @@ int64_t prompt_tiles(int32_t n_seq, int32_t n_tokens) { return (int64_t)n_tokens
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 int64_t prompt_info_bytes(int32_t n_seq, int32_t n_tokens, int32_t n_kv_heads) {
-    return round256(prompt_tiles(n_seq, n_tokens) * n_kv_heads * 16);
+    return round256(prompt_tiles(n_seq, n_tokens) * n_kv_heads * 4);
 }
 
 int64_t logprobs_chunks(int32_t n_rows, int64_t n_vocab, int eb) {

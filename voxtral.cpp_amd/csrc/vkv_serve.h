@@ -73,7 +73,7 @@ struct PromptArgs {
     int64_t n_tiles;       // key tiles of a kv head
     int64_t n_slots;       // query tiles of a kv head
     float scale;
-    int32_t *info;         // [kv head][tile][4]: exponents of K and V, whether V holds what is not finite
+    int32_t *info;         // [kv head][tile]: exponents of K and V, whether V holds what is not finite
     uint8_t *data;         // [kv head][tile]: the tile's matrix operands
 };
 
