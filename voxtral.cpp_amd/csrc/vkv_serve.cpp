@@ -148,7 +148,8 @@ int64_t logprobs_chunks(int32_t n_rows, int64_t n_vocab, int eb) {
     return (n_vocab + 16 / eb - 1 + per - 1) / per;
 }
 
-int64_t logprobs_stats_bytes(int64_t n_rows, int64_t chunks) { return n_rows * chunks * 16; }
+// (maximum, sum, weighted sum) of each wave
+int64_t logprobs_stats_bytes(int64_t n_rows, int64_t chunks) { return n_rows * chunks * 4 * 16; }
 
 }  // namespace
 

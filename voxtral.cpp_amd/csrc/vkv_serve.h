@@ -90,7 +90,7 @@ struct LogprobsArgs {
     float *logprob, *entropy;
     int32_t *top_ids;
     float *top_logprobs;
-    float *stats;                       // [row][chunk][4]: maximum, sum, weighted sum
+    float *stats;                       // [row][chunk][4 waves][4]: maximum, sum, weighted sum
     unsigned long long *keys;           // [row][chunk][n_top]
 };
 
