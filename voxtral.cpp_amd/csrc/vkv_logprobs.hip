@@ -8,6 +8,7 @@
 // lists.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 
 #include "vkv_serve.h"
@@ -18,8 +19,13 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kThreads = 256;
+// Pieces: 2 blocks per thread where that makes few work groups (a row or a
+// few: the time is latency), else 32 elements per thread, as many pieces per
+// work group as leave kManyGroups of them.
+constexpr int kBlocksFew = 2;
+constexpr int64_t kFewGroups = 1024, kManyGroups = 1024, kTurnsMost = 8;
 constexpr int kWaves = kThreads / 64;
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // Values in order as unsigned numbers: NaN above all, -0 beside 0.  An
 // element's key is its value's number above its index counted down, so keys
@@ -56,48 +62,78 @@ __device__ __forceinline__ float wave_sum(float x) {
     return wave_reduce(x, [](float a, float b) { return a + b; });
 }
 
-// A number that n of the wave's 64 numbers reach, and few more (0 where n are
-// not above 0): bit by bit from the top.
-template <typename N> __device__ __forceinline__ N nth_of_wave(N x, int n) {
+// A number that n of the work group's numbers (one per thread, in LDS) reach,
+// and few more (0 where n are not above 0): bit by bit from the top, each wave
+// for itself.
+template <typename N> __device__ __forceinline__ N nth_of_group(const N *x, int n) {
+    N mine[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mine[w] = x[w * 64 + (threadIdx.x & 63)];
     N t = 0;
     for (int bit = 8 * (int)sizeof(N) - 1; bit >= 0; --bit) {
         const N up = t | (N)1 << bit;
-        const int c = __popcll(__ballot(x >= up));
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) c += __popcll(__ballot(mine[w] >= up));
         if (c >= n) t = up;
-        if (c >= n && c <= n + 6) break;
+        if (c >= n && c <= n + n / 4) break;
     }
     return t;
 }
 
-constexpr int kListMax = 1024;
+// Keys of a few elements, a piece of the list for each wave; a few words
+// behind a piece are read, not used.
+constexpr int kPiece = 256;
+struct List {
+    u64 key[kWaves][kPiece];
+    u64 more[4];
+    __attribute__((aligned(16))) int count[kWaves];
+};
+
+// The wave's elements for which `take` holds go to its piece, as far as it has
+// room; `kept` counts them all.
+template <typename Take, typename Key> __device__ __forceinline__ void put(List &list, int &kept, Take take, Key key) {
+    const u64 on = __ballot(take);
+    if (on == 0) return;
+    const int at = kept + __builtin_amdgcn_mbcnt_hi((unsigned)(on >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)on, 0));
+    if (take && at < kPiece) list.key[threadIdx.x >> 6][at] = key();
+    kept += __popcll(on);
+}
 
 // The list's n largest in falling order at out[0, n), 0 where there are fewer;
-// keys of a list are distinct.  The list has room for seven more.
-__device__ __forceinline__ void rank(const u64 *list, int c, int n, u64 *out) {
-    for (int i = threadIdx.x; i < c; i += kThreads) {
-        const u64 k = list[i];
+// its keys are distinct.  A barrier is between the list's writing and this.
+__device__ __forceinline__ void rank(const List &list, int n, u64 *out) {
+    const int4 c = *(const int4 *)list.count;
+    const int to1 = c.x, to2 = to1 + c.y, to3 = to2 + c.z, total = to3 + c.w, most = max(max(c.x, c.y), max(c.z, c.w));
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+        const int w = (i >= to1) + (i >= to2) + (i >= to3);
+        const u64 k = list.key[w][i - (w == 0 ? 0 : w == 1 ? to1 : w == 2 ? to2 : to3)];
         int above = 0;
-        for (int j = 0; j < c; j += 8) {
-            u64 x[8];
+        for (int j = 0; j < most; j += 4) {
+            u64 x[kWaves][4];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) x[q] = list[j + q];
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int q = 0; q < 8; ++q) above += j + q < c && x[q] > k;
+                for (int v = 0; v < kWaves; ++v) x[v][q] = list.key[v][j + q];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                above += (j + q < c.x && x[0][q] > k) + (j + q < c.y && x[1][q] > k) + (j + q < c.z && x[2][q] > k) +
+                         (j + q < c.w && x[3][q] > k);
         }
         if (above < n) out[above] = k;
     }
-    for (int i = c + threadIdx.x; i < n; i += kThreads) out[i] = 0;
+    for (int i = total + threadIdx.x; i < n; i += kThreads) out[i] = 0;
 }
 
-// The n largest keys one after the other, each the largest below the last: for
-// chunks with so many equal values, or NaN, that a list does not hold them.
-template <int PER, typename Key> __device__ __forceinline__ void pick(Key key, int n, u64 *wave_best, u64 *out) {
+// The n largest of the row's elements [from, to) one after the other, each the
+// largest below the last: for chunks with so many equal values that a list
+// does not hold them, or NaN.
+template <typename T> __device__ __noinline__ void pick(const T *x, int64_t from, int64_t to, int n, u64 *wave_best, u64 *out) {
     u64 last = ~0ull;
     for (int r = 0; r < n; ++r) {
         u64 best = 0;
-#pragma unroll 4
-        for (int i = 0; i < PER; ++i) {
-            const u64 k = key(i);
+        for (int64_t i = from + threadIdx.x; i < to; i += kThreads) {
+            const u64 k = key_of((float)x[i], (unsigned)i);
             if (k < last && k > best) best = k;
         }
 #pragma unroll
@@ -114,125 +150,154 @@ template <int PER, typename Key> __device__ __forceinline__ void pick(Key key, i
     }
 }
 
-template <typename T, int BLOCKS> struct Chunk {
-    static constexpr int per_block = 16 / (int)sizeof(T);      // elements of a 16-byte block
-    static constexpr int per_thread = BLOCKS * per_block;
-};
-
-// A chunk: BLOCKS blocks of 16 bytes per thread, counted from the 16-byte
-// boundary at or below the row's first element.
+// A work group takes `turns` pieces of BLOCKS 16-byte blocks per thread,
+// counted from the 16-byte boundary at or below the row's first element; the
+// next piece is on its way while one is worked on.
 //
-// The n-th largest of a wave's 64 lane maxima is reached by n elements at
-// least, so nothing below the largest such value of the four waves is among
-// the chunk's n largest; what is not below it, a few more than n elements as a
-// rule, goes to a list that is ranked by counting.
+// A value that n of the 256 threads' maxima reach is reached by n elements at
+// least, so nothing below it is among the n largest.  Found once, in the first
+// piece, it is the limit for all: what is not below it, a few more than n
+// elements per piece as a rule, goes to a list that is ranked by counting.
 template <typename T, int BLOCKS>
 __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
-    constexpr int EB = Chunk<T, BLOCKS>::per_block, PER = Chunk<T, BLOCKS>::per_thread;
-    __shared__ u64 list[kListMax + 7];
+    constexpr int EB = 16 / (int)sizeof(T);     // elements of a block
+    constexpr int PER = BLOCKS * EB;            // of a thread and piece
+    constexpr int PIECE = kThreads * PER;
+    __shared__ List list;
     __shared__ u64 wave_best[kWaves];
-    __shared__ unsigned wave_t[kWaves];
-    __shared__ int count, wave_odd[kWaves];
+    __shared__ unsigned best[kThreads];
+    __shared__ int wave_odd[kWaves];
     const int tid = threadIdx.x, chunk = blockIdx.x, row = blockIdx.y;
     const T *x = (const T *)a.logits + (int64_t)row * a.row_stride;
     const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-    if (tid == 0) count = 0;
-
-    // element i of block b is the row's element first + b kThreads EB + i
-    const int64_t first = ((int64_t)chunk * BLOCKS * kThreads + tid) * EB - shift;
-    const int64_t chunk0 = (int64_t)chunk * BLOCKS * kThreads * EB - shift;
-    float v[PER];
-    if (chunk0 >= 0 && chunk0 + (int64_t)BLOCKS * kThreads * EB <= a.n_vocab) {
-        uint4 y[BLOCKS];
+    const int vocab = a.n_vocab;
+    const int chunk0 = (int)((int64_t)chunk * a.turns * PIECE - shift);
+    const int begin = max(chunk0, 0), end = (int)min((int64_t)chunk0 + (int64_t)a.turns * PIECE, (int64_t)vocab);
+    // (the first element of block b of a piece: piece + (b kThreads + tid) EB)
+    auto load = [&](int piece, uint4 *y) {
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) y[b] = *(const uint4 *)(x + first + b * kThreads * EB);
+        for (int b = 0; b < BLOCKS; ++b) {
+            const int e = piece + (b * kThreads + tid) * EB;
+            if (e >= 0 && e + EB <= vocab) y[b] = *(const uint4 *)(x + e);
+        }
+    };
+    uint4 next[BLOCKS];
+    load(chunk0, next);
+    float m = -INFINITY, s = 0.0f, t = 0.0f, limit = -INFINITY;
+    int kept = 0;
+    for (int piece = chunk0; piece < end; piece += PIECE) {
+        float v[PER];
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-            for (int i = 0; i < EB; ++i) v[b * EB + i] = (float)((const T *)&y[b])[i];
-    } else {
+            for (int i = 0; i < EB; ++i) v[b * EB + i] = (float)((const T *)&next[b])[i];
+        if (piece < 0 || piece + PIECE > vocab) {
+            // the row's ends: blocks that are not all its own, element by element
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-            const int64_t e = first + b * kThreads * EB;
-            if (e >= 0 && e + EB <= a.n_vocab) {
-                const uint4 y = *(const uint4 *)(x + e);
+            for (int b = 0; b < BLOCKS; ++b) {
+                const int e = piece + (b * kThreads + tid) * EB;
+                if (!(e >= 0 && e + EB <= vocab))
 #pragma unroll
-                for (int i = 0; i < EB; ++i) v[b * EB + i] = (float)((const T *)&y)[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < EB; ++i) v[b * EB + i] = e + i >= 0 && e + i < a.n_vocab ? (float)x[e + i] : -INFINITY;
+                    for (int i = 0; i < EB; ++i) v[b * EB + i] = e + i >= 0 && e + i < vocab ? (float)x[e + i] : -INFINITY;
             }
         }
-    }
-    float mine = v[0];
+        if (piece + PIECE < end) load(piece + PIECE, next);
+        float of_block[BLOCKS], mine = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < PER; ++i) mine = fmaxf(mine, v[i]);
-    const float m = wave_max(mine);
-    const float ref = m > -INFINITY ? m : 0.0f;
-    float s = 0.0f, t = 0.0f;
+        for (int b = 0; b < BLOCKS; ++b) {
+            of_block[b] = v[b * EB];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const float d = v[i] - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
-        s += e;
-        // (below -200 the exponential is 0: no infinity times 0)
-        t = fmaf(e, fmaxf(d, -200.0f), t);
+            for (int i = 1; i < EB; ++i) of_block[b] = fmaxf(of_block[b], v[b * EB + i]);
+            mine = fmaxf(mine, of_block[b]);
+        }
+        const float m_new = fmaxf(m, wave_max(mine));
+        const float ref = m_new > -INFINITY ? m_new : 0.0f;
+        // the sums so far move to the new maximum (without a term: none)
+        if (m_new > m && s != 0.0f) {
+            const float d = (m - ref) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+            t = f != 0.0f ? f * fmaf(d, s, t) : 0.0f;
+            s *= f;
+        }
+        m = m_new;
+        // exp(x - ref) = 2^d, d = x log2 e - c in one rounding; what c's own
+        // lacks is the same for every term and comes off the sums
+        const float c = ref * kLog2e;
+        float lack = fmaf(ref, kLog2e, -c), s1 = 0.0f, t1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const float d = fmaf(v[i], kLog2e, -c), e = __builtin_amdgcn_exp2f(d);
+            s1 += e;
+            t1 = fmaf(e, d, t1);
+        }
+        if (__any(!(fabsf(t1) <= FLT_MAX))) {
+            // a logit of -inf (0 times the logarithm of 0 is 0), or a c beyond
+            // the range: d from the difference
+            lack = s1 = t1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const float d = (v[i] - ref) * kLog2e, e = __builtin_amdgcn_exp2f(d);
+                s1 += e;
+                t1 = fmaf(e, fmaxf(d, -200.0f), t1);
+            }
+        }
+        t1 = fmaf(-lack, s1, t1);
+        lack = fmaf(-lack, kLn2, 1.0f);
+        s = fmaf(s1, lack, s);
+        t = fmaf(t1, lack, t);          // in log2 units
+        if (a.n_top == 0) continue;
+        if (!(limit > -INFINITY)) {
+            __syncthreads();
+            best[tid] = order_of(mine);
+            __syncthreads();
+            limit = value_of(nth_of_group(best, a.n_top));
+        }
+        auto at = [&](int i) { return piece + ((i / EB) * kThreads + tid) * EB + i % EB; };
+        if (limit > -INFINITY) {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+                if (__any(of_block[b] >= limit))
+#pragma unroll
+                    for (int i = b * EB; i < (b + 1) * EB; ++i)
+                        put(list, kept, v[i] >= limit, [&] { return key_of(v[i], (unsigned)at(i)); });
+        } else {
+            // fewer than n above -inf: they, and the chunk's first n for those of -inf that rank
+#pragma unroll 1
+            for (int b = 0; b < BLOCKS; ++b)
+                for (int i = 0; i < EB; ++i) {
+                    const int e = piece + (b * kThreads + tid) * EB + i;
+                    const float y = e >= 0 && e < vocab ? (float)x[e] : -INFINITY;
+                    put(list, kept, e >= 0 && e < vocab && (y > -INFINITY || e - begin < a.n_top),
+                        [&] { return key_of(y, (unsigned)e); });
+                }
+        }
     }
     s = wave_sum(s);
     t = wave_sum(t);
     if ((tid & 63) == 0) {
-        float *st = a.stats + (((int64_t)row * a.n_chunks + chunk) * kWaves + (tid >> 6)) * 4;
-        st[0] = m;
-        st[1] = s;
-        st[2] = t;
-        wave_odd[tid >> 6] = s != s;     // NaN, or +inf
+        *((float4 *)a.stats + ((int64_t)row * a.n_chunks + chunk) * kWaves + (tid >> 6)) = float4{m, s, t * kLn2, 0.0f};
+        list.count[tid >> 6] = min(kept, kPiece);
+        wave_odd[tid >> 6] = s != s || kept > kPiece;   // NaN or +inf, or a full list
     }
     if (a.n_top == 0) return;
-    const unsigned nth = nth_of_wave(order_of(mine), a.n_top);
-    if ((tid & 63) == 0) wave_t[tid >> 6] = nth;
-    __syncthreads();
-    unsigned least = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) least = wave_t[w] > least ? wave_t[w] : least;
-    const float limit = value_of(least);
-    const int64_t left = a.n_vocab - first;
-    auto at = [&](int i) { return (i / EB) * kThreads * EB + i % EB; };      // from first
-    if (limit > -INFINITY) {
-        if (mine >= limit) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (v[i] >= limit) {
-                    const int p = atomicAdd(&count, 1);
-                    if (p < kListMax) list[p] = key_of(v[i], (unsigned)(first + at(i)));
-                }
-        }
-    } else {
-        // fewer than n above -inf: they, and the first n of the chunk for those of -inf that rank
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if ((v[i] > -INFINITY || first + at(i) - max(chunk0, (int64_t)0) < a.n_top) && first + at(i) >= 0 && at(i) < left) {
-                const int p = atomicAdd(&count, 1);
-                if (p < kListMax) list[p] = key_of(v[i], (unsigned)(first + at(i)));
-            }
-    }
     __syncthreads();
     u64 *out = a.keys + ((int64_t)row * a.n_chunks + chunk) * a.n_top;
-    if (wave_odd[0] | wave_odd[1] | wave_odd[2] | wave_odd[3] || count > kListMax)
-        pick<PER>([&](int i) -> u64 { return first + at(i) >= 0 && at(i) < left ? key_of(v[i], (unsigned)(first + at(i))) : 0; },
-                  a.n_top, wave_best, out);
+    if (wave_odd[0] | wave_odd[1] | wave_odd[2] | wave_odd[3])
+        pick(x, begin, end, a.n_top, wave_best, out);
     else
-        rank(list, count, a.n_top, out);
+        rank(list, a.n_top, out);
 }
 
-constexpr int kJoinPer = 4;      // keys of the chunks' lists per thread and turn
+// keys of the chunks' lists per thread and turn: with the largest so far, a
+// wave's fit its piece
+constexpr int kJoinPer = 3;
 
 // A work group per row.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
-    __shared__ u64 list[kThreads * kJoinPer + kLogprobsMaxTop + 7];
-    __shared__ u64 wave_t[kWaves];
+    __shared__ List list;
+    __shared__ u64 bests[kThreads];
     __shared__ u64 top[kLogprobsMaxTop];
     __shared__ float red[kWaves][4];
-    __shared__ int count;
     const int tid = threadIdx.x, row = blockIdx.x;
     const float4 *st = (const float4 *)a.stats + (int64_t)row * a.n_chunks * kWaves;
     const int n_stats = a.n_chunks * kWaves;
@@ -287,20 +352,20 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
         u64 best = 0;
 #pragma unroll
         for (int i = 0; i < kJoinPer; ++i) best = k[i] > best ? k[i] : best;
-        const u64 nth = nth_of_wave(best, a.n_top);
-        __syncthreads();
-        if (tid == 0) count = 0;
-        if ((tid & 63) == 0) wave_t[tid >> 6] = nth;
-        __syncthreads();
         u64 least = 1;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) least = wave_t[w] > least ? wave_t[w] : least;
-#pragma unroll
-        for (int i = 0; i < kJoinPer; ++i)
-            if (k[i] >= least) list[atomicAdd(&count, 1)] = k[i];
-        if (base && tid < a.n_top && top[tid]) list[atomicAdd(&count, 1)] = top[tid];
         __syncthreads();
-        rank(list, count, a.n_top, top);
+        if (n_keys > kThreads) {        // (else the list takes them all)
+            bests[tid] = best;
+            __syncthreads();
+            least = max(nth_of_group(bests, a.n_top), (u64)1);
+        }
+        int kept = 0;
+#pragma unroll
+        for (int i = 0; i < kJoinPer; ++i) put(list, kept, k[i] >= least, [&] { return k[i]; });
+        if (base) put(list, kept, tid < a.n_top && top[tid] >= least, [&] { return top[tid]; });
+        if ((tid & 63) == 0) list.count[tid >> 6] = kept;
+        __syncthreads();
+        rank(list, a.n_top, top);
     }
     __syncthreads();
     s = red[0][1] + red[1][1] + red[2][1] + red[3][1];
@@ -322,8 +387,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
 
 template <typename T> hipError_t run(const LogprobsArgs &a, int blocks, hipStream_t st) {
     const dim3 grid((unsigned)a.n_chunks, (unsigned)a.n_rows);
-    if (blocks == 2)
-        k_logprobs_part<T, 2><<<grid, kThreads, 0, st>>>(a);
+    if (blocks == kBlocksFew)
+        k_logprobs_part<T, kBlocksFew><<<grid, kThreads, 0, st>>>(a);
     else
         k_logprobs_part<T, sizeof(T) == 4 ? 8 : 4><<<grid, kThreads, 0, st>>>(a);
     k_logprobs_join<T><<<(unsigned)a.n_rows, kThreads, 0, st>>>(a);
@@ -332,13 +397,20 @@ template <typename T> hipError_t run(const LogprobsArgs &a, int blocks, hipStrea
 
 }  // namespace
 
-int logprobs_blocks(int n_rows, int64_t n_vocab, int elem_bytes) {
-    const int64_t small = n_rows * ((n_vocab * elem_bytes / 16 + 1) / (2 * kThreads) + 1);
-    return small <= 1024 ? 2 : elem_bytes == 4 ? 8 : 4;
+LogprobsPlan logprobs_plan(int n_rows, int64_t n_vocab, int elem_bytes) {
+    // blocks of a row, wherever in a block it begins
+    const int64_t blocks = (n_vocab + 2 * (16 / elem_bytes) - 2) / (16 / elem_bytes);
+    LogprobsPlan p;
+    const int64_t small = (blocks + kBlocksFew * kThreads - 1) / (kBlocksFew * kThreads);
+    p.blocks = n_rows * small <= kFewGroups ? kBlocksFew : elem_bytes == 4 ? 8 : 4;
+    const int64_t pieces = (blocks + p.blocks * kThreads - 1) / (p.blocks * kThreads);
+    p.turns = (int32_t)std::min<int64_t>(std::max<int64_t>(n_rows * pieces / kManyGroups, 1), std::min<int64_t>(pieces, kTurnsMost));
+    p.chunks = (int32_t)((pieces + p.turns - 1) / p.turns);
+    return p;
 }
 
 hipError_t launch_logprobs(int dtype, const LogprobsArgs &a, hipStream_t st) {
-    const int blocks = logprobs_blocks(a.n_rows, a.n_vocab, dtype == VKV_DTYPE_F32 ? 4 : 2);
+    const int blocks = logprobs_plan(a.n_rows, a.n_vocab, dtype == VKV_DTYPE_F32 ? 4 : 2).blocks;
     if (dtype == VKV_DTYPE_F16) return run<_Float16>(a, blocks, st);
     if (dtype == VKV_DTYPE_BF16) return run<__bf16>(a, blocks, st);
     return run<float>(a, blocks, st);

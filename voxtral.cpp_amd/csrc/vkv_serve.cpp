@@ -143,11 +143,6 @@ int64_t prompt_info_bytes(int32_t n_seq, int32_t n_tokens, int32_t n_kv_heads) {
     return round256(prompt_tiles(n_seq, n_tokens) * n_kv_heads * 4);
 }
 
-int64_t logprobs_chunks(int32_t n_rows, int64_t n_vocab, int eb) {
-    const int64_t per = (int64_t)logprobs_blocks(n_rows, n_vocab, eb) * 256 * (16 / eb);
-    return (n_vocab + 16 / eb - 1 + per - 1) / per;
-}
-
 // (maximum, sum, weighted sum) of each wave
 int64_t logprobs_stats_bytes(int64_t n_rows, int64_t chunks) { return n_rows * chunks * 4 * 16; }
 
@@ -336,7 +331,7 @@ vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const
 size_t vkv_logprobs_workspace(int32_t n_rows, int64_t n_vocab, int32_t n_top) {
     if (n_rows < 0 || n_vocab < 1 || n_vocab > 1 << 30 || n_top < 0 || n_top > kLogprobsMaxTop) return 0;
     int64_t most = 0;
-    for (int eb : {2, 4}) most = std::max(most, logprobs_chunks(n_rows, n_vocab, eb));
+    for (int eb : {2, 4}) most = std::max<int64_t>(most, logprobs_plan(n_rows, n_vocab, eb).chunks);
     return (size_t)(logprobs_stats_bytes(n_rows, most) + n_rows * most * n_top * 8);
 }
 
@@ -359,11 +354,12 @@ vkv_status vkv_logprobs(int32_t dtype, const void *logits, int64_t row_stride, i
             if (vkv_status s = check_ints(what, p)) return s;
     if (!aligned(tokens, 4) || !aligned(logprob, 4) || !aligned(entropy, 4))
         return bad("%s: int32 and f32 arrays must be 4-byte aligned", what);
-    const int64_t chunks = logprobs_chunks(n_rows, n_vocab, eb);
+    const LogprobsPlan plan = logprobs_plan(n_rows, n_vocab, eb);
+    const int64_t chunks = plan.chunks;
     const int64_t stats = logprobs_stats_bytes(n_rows, chunks), need = stats + n_rows * chunks * n_top * 8;
     if ((int64_t)workspace_bytes < need) return small_ws(what, workspace_bytes, (size_t)need);
     if (!workspace || !aligned(workspace, 16)) return bad("%s: workspace null or not 16-byte aligned", what);
-    LogprobsArgs a{logits, row_stride, n_rows, (int32_t)n_vocab, n_top, (int32_t)chunks, tokens, logprob, entropy,
+    LogprobsArgs a{logits, row_stride, n_rows, (int32_t)n_vocab, n_top, plan.chunks, plan.turns, tokens, logprob, entropy,
                    top_ids, top_logprobs, (float *)workspace, (unsigned long long *)((uint8_t *)workspace + stats)};
     StreamDevice on(as_stream(hip_stream));
     const hipError_t e = launch_logprobs(dtype, a, as_stream(hip_stream));

@@ -85,7 +85,7 @@ constexpr int kLogprobsMaxTop = 32;
 struct LogprobsArgs {
     const void *logits;
     int64_t row_stride;
-    int32_t n_rows, n_vocab, n_top, n_chunks;
+    int32_t n_rows, n_vocab, n_top, n_chunks, turns;
     const int32_t *tokens;
     float *logprob, *entropy;
     int32_t *top_ids;
@@ -94,8 +94,11 @@ struct LogprobsArgs {
     unsigned long long *keys;           // [row][chunk][n_top]
 };
 
-// 16-byte blocks of a row per work group and chunk for a call
-int logprobs_blocks(int n_rows, int64_t n_vocab, int elem_bytes);
+// 16-byte blocks per thread and piece, pieces per chunk, chunks per row
+struct LogprobsPlan {
+    int32_t blocks, turns, chunks;
+};
+LogprobsPlan logprobs_plan(int n_rows, int64_t n_vocab, int elem_bytes);
 hipError_t launch_logprobs(int dtype, const LogprobsArgs &a, hipStream_t st);
 
 }  // namespace vkv
