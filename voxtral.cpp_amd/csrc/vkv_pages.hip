@@ -328,127 +328,149 @@ __device__ __forceinline__ float wave_max(float x) {
     return x;
 }
 
-// One work group per new token that opens its page's run of tokens, and four
-// (K or V, head) units; the other tokens' work groups end at once.  A wave
-// owns one unit of the page: largest magnitude of the run's rows, the scale
-// they need, then the codes of every 16-token block of the page that changes.
-// Lane (g, c) of a block: K rows 4 j + g, dims [c D/16, (c + 1) D/16); V rows
-// 4 g + j, dims 16 t + c, which is the block's stored order.
-template <typename T, int FMT, int D>
-__global__ __launch_bounds__(256) void k_pages_append(AppendPagesArgs a) {
-    constexpr int N = D / 16;
-    __shared__ int win[256];    // last token of the run for each slot of the page, -1: none
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    const int S = a.page_size;
-    const int slot = a.slots[t];
-    if (slot < 0 || slot >= a.n_slots) return;
-    const int page = slot / S;
-    if (t > 0) {
-        const int before = a.slots[t - 1];
-        if (before >= 0 && before < a.n_slots && before / S == page) return;
-    }
-    if (tid < S) win[tid] = -1;
-    __syncthreads();
-    for (int i0 = t;; i0 += 256) {
-        const int i = i0 + tid;
-        const int s = i < a.n_tokens ? a.slots[i] : -1;
-        const bool in = s >= 0 && s < a.n_slots && s / S == page;
-        // the run ends at the first token of another page
-        __shared__ int end;
-        if (tid == 0) end = i0 + 256;
-        __syncthreads();
-        if (!in) atomicMin(&end, i);
-        __syncthreads();
-        const int stop = end;
-        if (i < stop) atomicMax(&win[s - page * S], i);
-        __syncthreads();
-        if (stop < i0 + 256) break;
-    }
-    const int unit = blockIdx.y * 4 + (tid >> 6);
-    if (unit >= 2 * a.n_kv_heads) return;
-    const bool is_v = unit >= a.n_kv_heads;
-    const int head = is_v ? unit - a.n_kv_heads : unit;
-    const int g = lane >> 4, c = lane & 15;
-    const T *src = (const T *)(is_v ? a.v : a.k) + head * D + (is_v ? c : c * N);
-    const int step = is_v ? 16 : 1;      // between a lane's dims
-    const int64_t ph = (int64_t)page * a.n_kv_heads + head;
-    uint8_t *codes = (is_v ? a.v_codes : a.k_codes) + ph * ((int64_t)S * D);
-    float *scale = (is_v ? a.v_scale : a.k_scale) + ph;
-
-    auto row_of = [&](int b, int j) { return win[16 * b + (is_v ? 4 * g + j : 4 * j + g)]; };
-    float amax = 0.0f;
-    for (int b = 0; b < S / 16; ++b)
+// Eight (or four) neighbouring values of a row, as they are stored.
+template <typename T, int N> struct Raw {
+    uint4 w[(N * sizeof(T) + 15) / 16];
+    __device__ void load(const T *p) {
+        if constexpr (N * sizeof(T) >= 16) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = row_of(b, j);
-            if (i < 0) continue;
-            const T *p = src + (int64_t)i * a.row_stride;
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const float x = to_f32(p[n * step]);
-                amax = fmaxf(amax, is_finite(x) ? fabsf(x) : 0.0f);
-            }
+            for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i) w[i] = ((const uint4 *)p)[i];
+        } else {
+            const uint2 x = *(const uint2 *)p;
+            w[0].x = x.x;
+            w[0].y = x.y;
         }
-    amax = wave_max(amax);
-    int e = scale_exponent<FMT>(amax);
-    // a page begins with its slot 0: what it held before does not count
-    const bool fresh = win[0] >= 0;
-    float down = 1.0f;
-    if (!fresh) {
-        const int old = exponent_of(*scale);
-        if (e > old) down = exp2_int(max(old - e, -126)); else e = old;
     }
-    const bool grown = down != 1.0f;
-    const float inv = exp2_int(-e);
-    if (lane == 0) *scale = exp2_int(e);
+    __device__ float operator[](int i) const { return to_f32(((const T *)w)[i]); }
+};
 
-    for (int b = 0; b < S / 16; ++b) {
-        bool any = false;
+// The run of tokens that a page's rows come in: the work group of the run's
+// first token does it all; `looks` tokens are a work group's to look at for
+// first ones (one where the tokens are few, so that each has a work group of
+// its own; a page's worth where most tokens are in the middle of a run).
+//
+// A wave owns one 16-token block of one (page, K or V, head), so a block's
+// rows are read once and stay in registers between the search for the largest
+// magnitude and the rounding; S / 16 waves share a page and meet in LDS.  Lane
+// (g, c) has rows 4 g + j and dims [c D/16, (c + 1) D/16): four tokens of a
+// dim are a word of V's stored order.
+template <typename T, int FMT, int D>
+__global__ __launch_bounds__(1024) void k_pages_append(AppendPagesArgs a) {
+    constexpr int N = D / 16;
+    __shared__ int win[16][16];     // a wave's: last token of the run for each slot of its block, -1: none
+    __shared__ float top[16];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int S = a.page_size, blocks = S / 16, units = (int)blockDim.x / 64 / blocks;
+    const int unit = blockIdx.y * units + wave / blocks, b = wave % blocks;
+    const bool busy = unit < 2 * a.n_kv_heads;
+    const bool is_v = unit >= a.n_kv_heads;
+    const int head = busy ? is_v ? unit - a.n_kv_heads : unit : 0;
+    const int g = lane >> 4, c = lane & 15;
+    auto slot_at = [&](int t) { return t >= 0 && t < a.n_tokens ? a.slots[t] : -1; };
+    auto page_of = [&](int s) { return s >= 0 && s < a.n_slots ? s / S : -1; };
+    // first tokens of their page among those this work group looks at
+    const int t0 = blockIdx.x * a.looks;
+    const int slot0 = slot_at(t0 + lane), before0 = slot_at(t0 + lane - 1);
+    const int page0 = page_of(slot0);
+    unsigned long long firsts = __ballot(lane < a.looks && page0 >= 0 && page0 != page_of(before0));
+    for (; firsts; firsts &= firsts - 1) {
+        const int bit = __ffsll(firsts) - 1, t = t0 + bit;
+        const int page = __builtin_amdgcn_readlane(page0, bit);
+        // the run, which ends at the first token of another page: each wave
+        // for its own block
+        if (lane < 16) win[wave][lane] = -1;
+        bool fresh = false;      // a page begins with its slot 0: what it held before does not count
+        for (int i = t + lane, slot = bit == 0 ? slot0 : slot_at(i);;) {
+            const unsigned long long out = __ballot(page_of(slot) != page);
+            const int n = out ? __ffsll(out) - 1 : 64;
+            const int offset = slot - page * S;
+            fresh |= __any(lane < n && offset == 0);
+            if (lane < n && offset >> 4 == b) atomicMax(&win[wave][offset & 15], i);
+            if (out) break;
+            i += 64;
+            slot = slot_at(i);
+        }
+        const int64_t ph = (int64_t)page * a.n_kv_heads + head;
+        uint8_t *codes = (is_v ? a.v_codes : a.k_codes) + ph * ((int64_t)S * D) + b * (16 * D);
+        float *scale = (is_v ? a.v_scale : a.k_scale) + ph;
+        const float scale_old = *scale;
         int rows[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            rows[j] = row_of(b, j);
-            any |= rows[j] >= 0;
-        }
-        if (!any && !grown) continue;
-        float x[4][N];
+        for (int j = 0; j < 4; ++j) rows[j] = busy ? win[wave][4 * g + j] : -1;
+        const T *src = (const T *)(is_v ? a.v : a.k) + head * D + c * N;
+        Raw<T, N> x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const T *p = src + (int64_t)max(rows[j], 0) * a.row_stride;
+        for (int j = 0; j < 4; ++j)
+            if (rows[j] >= 0) x[j].load(src + (int64_t)rows[j] * a.row_stride);
+        // words of the block as it is: K by row, V by dim, for what is kept of them
+        unsigned old[4][N / 4];
+        const bool whole = rows[0] >= 0 && rows[1] >= 0 && rows[2] >= 0 && rows[3] >= 0;
+        if (busy && !whole) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                old[i / (N / 4)][i % (N / 4)] =
+                    is_v ? ((const unsigned *)codes)[(((c * N + i) % 16) * 4 + g) * N + (c * N + i) / 16]
+                         : ((const unsigned *)(codes + (4 * g + i / (N / 4)) * D + c * N))[i % (N / 4)];
+        }
+        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
             if (rows[j] >= 0)
 #pragma unroll
-                for (int n = 0; n < N; ++n) x[j][n] = to_f32(p[n * step]) * inv;
+                for (int n = 0; n < N; ++n) {
+                    const float y = fabsf(x[j][n]);
+                    amax = fmaxf(amax, y <= FLT_MAX ? y : 0.0f);
+                }
+        amax = wave_max(amax);
+        if (blocks > 1) {
+            __syncthreads();
+            if (lane == 0) top[wave] = amax;
+            __syncthreads();
+            for (int i = 0; i < blocks; ++i) amax = fmaxf(amax, top[wave - b + i]);
         }
+        if (!busy) continue;
+        int e = scale_exponent<FMT>(amax);
+        float down = 1.0f;
+        if (!fresh) {
+            const int before = exponent_of(scale_old);
+            if (e > before) down = exp2_int(max(before - e, -126)); else e = before;
+        }
+        const bool grown = down != 1.0f;
+        const float inv = exp2_int(-e);
+        if (b == 0 && lane == 0) *scale = exp2_int(e);
         if (!is_v) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                unsigned *dst = (unsigned *)(codes + (int64_t)(16 * b + 4 * j + g) * D + c * N);
+            for (int j = 0; j < 4; ++j)
+                if (rows[j] >= 0 || grown) {
+                    unsigned w[N / 4];
 #pragma unroll
-                for (int n = 0; n < N / 4; ++n) {
-                    if (rows[j] >= 0)
-                        dst[n] = pack4<FMT>(x[j][4 * n], x[j][4 * n + 1], x[j][4 * n + 2], x[j][4 * n + 3]);
-                    else if (grown)
-                        dst[n] = rescale4<FMT>(dst[n], down);
+                    for (int n = 0; n < N / 4; ++n)
+                        w[n] = rows[j] >= 0 ? pack4<FMT>(x[j][4 * n] * inv, x[j][4 * n + 1] * inv, x[j][4 * n + 2] * inv,
+                                                         x[j][4 * n + 3] * inv)
+                                            : rescale4<FMT>(old[j][n], down);
+                    unsigned *dst = (unsigned *)(codes + (4 * g + j) * D + c * N);
+                    if constexpr (N == 8)
+                        *(uint2 *)dst = uint2{w[0], w[1]};
+                    else
+                        *dst = w[0];
                 }
-            }
         } else {
-            unsigned *dst = (unsigned *)(codes + (int64_t)b * 16 * D) + (c * 4 + g) * N;
             unsigned mask = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) mask |= rows[j] >= 0 ? 255u << 8 * j : 0u;
-            if (mask != 0 || grown) {
+            if (mask != 0 || grown)
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
-                    unsigned w = 0;
-                    if (mask != 0xffffffffu) {
-                        w = dst[n];
+                    unsigned y = pack4<FMT>(rows[0] >= 0 ? x[0][n] * inv : 0.0f, rows[1] >= 0 ? x[1][n] * inv : 0.0f,
+                                            rows[2] >= 0 ? x[2][n] * inv : 0.0f, rows[3] >= 0 ? x[3][n] * inv : 0.0f);
+                    if (!whole) {
+                        unsigned w = old[n / (N / 4)][n % (N / 4)];
                         if (grown) w = rescale4<FMT>(w, down);
+                        y = (w & ~mask) | (y & mask);
                     }
-                    const unsigned y = pack4<FMT>(rows[0] >= 0 ? x[0][n] : 0.0f, rows[1] >= 0 ? x[1][n] : 0.0f,
-                                                  rows[2] >= 0 ? x[2][n] : 0.0f, rows[3] >= 0 ? x[3][n] : 0.0f);
-                    dst[n] = (w & ~mask) | (y & mask);
+                    ((unsigned *)codes)[(((c * N + n) % 16) * 4 + g) * N + (c * N + n) / 16] = y;
                 }
-            }
         }
     }
 }
@@ -785,8 +807,9 @@ template <typename T, int FMT, int D> hipError_t attn_launch(const PagedAttnArgs
 }
 
 template <typename T, int FMT, int D> hipError_t append_launch(const AppendPagesArgs &a, hipStream_t st) {
-    const dim3 grid((unsigned)a.n_tokens, (unsigned)((2 * a.n_kv_heads + 3) / 4));
-    k_pages_append<T, FMT, D><<<grid, 256, 0, st>>>(a);
+    const int waves = a.page_size / 16 > 4 ? a.page_size / 16 : 4, units = waves / (a.page_size / 16);
+    const dim3 grid((unsigned)((a.n_tokens + a.looks - 1) / a.looks), (unsigned)((2 * a.n_kv_heads + units - 1) / units));
+    k_pages_append<T, FMT, D><<<grid, 64 * waves, 0, st>>>(a);
     return hipGetLastError();
 }
 

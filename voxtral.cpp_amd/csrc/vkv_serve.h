@@ -35,7 +35,10 @@ struct AppendPagesArgs {
     const void *k, *v;
     int64_t row_stride;
     int32_t n_tokens, n_slots, page_size, n_kv_heads;
+    int32_t looks;         // tokens that a work group looks at for first ones of their page (<= 64)
 };
+// Up to so many tokens, an append has a work group (per few heads) for each.
+constexpr int kAppendAlone = 512;
 
 hipError_t launch_pages_append(int dtype, int code, int head_dim, const AppendPagesArgs &a, hipStream_t st);
 
