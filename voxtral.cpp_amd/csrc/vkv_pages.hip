@@ -88,8 +88,8 @@ __device__ __forceinline__ void map_token(const MapArgs &a, int t, int r, int po
     a.positions[t] = pos;
 }
 
-// One work group: the free stack is one list, and a step's lengths are a few
-// KB.  Pass 1 sums what the step moves and checks it; nothing is written
+// Any number of requests.  One work group: the free stack is one list, and a
+// step's lengths are a few KB.  Pass 1 sums what the step moves and checks it; nothing is written
 // before the whole step is known to fit.  Pass 2 pushes the returned pages,
 // pass 3 pops the taken ones; both spread the moved pages (not the requests)
 // over the threads, by a search in the scanned counts.
@@ -231,18 +231,177 @@ __global__ __launch_bounds__(kMapThreads) void k_page_map(MapArgs a) {
     }
 }
 
-// Slots and positions of many tokens, after k_page_map<true>.
+// inclusive sum over the wave
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);      // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // row_bcast 15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // row_bcast 31 into rows 2 and 3
+    return x;
+}
+
+// The same as k_page_map for as many requests as threads: a request is a
+// thread's from the first load to the last store, the three sums are scanned
+// together, and a step of single tokens (the usual one) needs no search and
+// two trips to memory, lengths and then pages.  The time is latency: 32
+// requests take one wave, whose barriers cost nothing.
+template <int THREADS, bool NOTOKENS>
+__global__ __launch_bounds__(THREADS) void k_page_map_small(MapArgs a) {
+    constexpr int WAVES = THREADS / 64;
+    __shared__ int upto[3][THREADS];        // inclusive sums: returned, taken, grown
+    __shared__ int from[3][THREADS];        // a request's first entry or position, less the sum before it
+    __shared__ int held_of[THREADS];
+    __shared__ __attribute__((aligned(16))) int of_wave[WAVES][4];
+    __shared__ float rough[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int n_free = *a.n_free;
+    const int shift = __builtin_ctz((unsigned)a.page_size);
+    const int64_t cap = (int64_t)a.table_stride << shift;
+    const bool mine = tid < a.n_req;
+    const int old_len = mine ? a.len_old[tid] : 0, new_len = mine ? a.len_new[tid] : 0;
+    const bool wrong = old_len < 0 || new_len < 0 || old_len > cap || new_len > cap;
+    const int round = a.page_size - 1;
+    const int held = (int)(((int64_t)old_len + round) >> shift), want = (int)(((int64_t)new_len + round) >> shift);
+    const int ret = max(held - want, 0), take = max(want - held, 0), grow = wrong ? 0 : max(new_len - old_len, 0);
+    int up[3] = {wave_scan(wrong ? 0 : ret), wave_scan(wrong ? 0 : take), wave_scan(grow)};
+    // the sums wrap only beyond what any step may move, and a rough sum tells
+    float r = wrong ? 0.0f : (float)ret + (float)take + (float)grow;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) r += __shfl_xor(r, d);
+    const bool many = __any(take > 1 || grow > 1);
+    if (lane == 63) {
+        of_wave[wave][0] = up[0];
+        of_wave[wave][1] = up[1];
+        of_wave[wave][2] = up[2];
+    }
+    const bool any_wrong = __any(wrong);
+    if (lane == 0) {
+        of_wave[wave][3] = (any_wrong ? 1 : 0) | (many ? 2 : 0);
+        rough[wave] = r;
+    }
+    __syncthreads();
+    int total[3] = {0, 0, 0}, flags = 0;
+    r = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const int4 x = *(const int4 *)of_wave[w];
+        if (w < wave) {
+            up[0] += x.x;
+            up[1] += x.y;
+            up[2] += x.z;
+        }
+        total[0] += x.x;
+        total[1] += x.y;
+        total[2] += x.z;
+        flags |= x.w;
+        r += rough[w];
+    }
+    // (max_tokens < 2^30, pages < 2^27 by the checks of the call)
+    bool bad = (flags & 1) || r > 1.5e9f || n_free < 0 || n_free > a.n_pages || total[0] > a.n_pages - n_free ||
+               total[2] > a.max_tokens;
+    const int n_ret = bad ? 0 : total[0];
+    const bool spread = (flags & 2) != 0 && !bad;
+    if (n_ret > 0 || spread) {
+        upto[0][tid] = up[0];
+        upto[1][tid] = up[1];
+        upto[2][tid] = up[2];
+        from[0][tid] = want - (up[0] - ret);
+        from[1][tid] = held - (up[1] - take);
+        from[2][tid] = old_len - (up[2] - grow);
+        held_of[tid] = held;
+        __syncthreads();
+    }
+    auto returned = [&](int j) {
+        const int q = upper_bound(upto[0], THREADS, j);
+        return a.table[(int64_t)q * a.table_stride + from[0][q] + j];
+    };
+    if (n_ret > 0) {    // the ids to be returned are checked before one of them is pushed
+        bool strange = false;
+        for (int j = tid; j < n_ret; j += THREADS) {
+            const int id = returned(j);
+            strange |= id < 0 || id >= a.n_pages;
+        }
+        bad = __syncthreads_or(strange);
+    }
+    const int status = bad ? 2 : total[1] > n_free + n_ret ? 1 : 0;
+    if (status) {       // nothing moves
+        if (mine) a.len_out[tid] = old_len;
+        for (int i = tid; i <= a.n_req; i += THREADS) a.cu_new[i] = 0;
+        if (!NOTOKENS)
+            for (int t = tid; t < a.max_tokens; t += THREADS) a.slots[t] = a.positions[t] = -1;
+        if (tid == 0) {
+            *a.n_free_out = n_free;
+            *a.status = status;
+        }
+        return;
+    }
+    if (n_ret > 0) {
+        for (int j = tid; j < n_ret; j += THREADS) a.free_pages[n_free + j] = returned(j);
+        __syncthreads();
+    }
+    const int top = n_free + n_ret, n_take = total[1], n_grow = total[2];
+    if (!spread) {
+        int page = -1;
+        if (take) page = a.free_pages[top - up[1]];
+        const int entry = old_len >> shift;
+        if (grow && !NOTOKENS) {
+            const int p = take ? page : a.table[(int64_t)tid * a.table_stride + entry];
+            a.slots[up[2] - 1] = (p << shift) + (old_len & round);
+            a.positions[up[2] - 1] = old_len;
+        }
+        if (take) a.table[(int64_t)tid * a.table_stride + held] = page;
+    } else {
+        for (int j = tid; j < n_take; j += THREADS) {
+            const int q = upper_bound(upto[1], THREADS, j);
+            a.table[(int64_t)q * a.table_stride + from[1][q] + j] = a.free_pages[top - 1 - j];
+        }
+        if (!NOTOKENS)
+            for (int t = tid; t < n_grow; t += THREADS) {
+                const int q = upper_bound(upto[2], THREADS, t), pos = from[2][q] + t, entry = pos >> shift;
+                // a new page's id straight from the stack
+                const int p = entry >= held_of[q] ? a.free_pages[top - 1 - (entry - from[1][q])]
+                                                  : a.table[(int64_t)q * a.table_stride + entry];
+                a.slots[t] = (p << shift) + (pos & round);
+                a.positions[t] = pos;
+            }
+    }
+    if (mine) {
+        a.cu_new[tid] = up[2] - grow;
+        a.len_out[tid] = new_len;
+    }
+    if (!NOTOKENS)
+        for (int t = n_grow + tid; t < a.max_tokens; t += THREADS) a.slots[t] = a.positions[t] = -1;
+    if (tid == 0) {
+        a.cu_new[a.n_req] = n_grow;
+        *a.n_free_out = top - n_take;
+        *a.status = 0;
+    }
+}
+
+constexpr int kMapOffsets = 4096;    // that k_map_tokens keeps in LDS
+
+// Slots and positions of many tokens, after the map itself, by a search in
+// the offsets.
 __global__ __launch_bounds__(256) void k_map_tokens(MapArgs a) {
-    const int n = a.n_req, total = a.cu_new[n];
+    __shared__ int cu[kMapOffsets];
+    const int n = a.n_req;
+    const int *offsets = a.cu_new;
+    if (n < kMapOffsets) {
+        for (int i = threadIdx.x; i <= n; i += 256) cu[i] = a.cu_new[i];
+        __syncthreads();
+        offsets = cu;
+    }
+    const int total = offsets[n];
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < a.max_tokens; t += (int64_t)gridDim.x * 256) {
         if (t >= total) {
             a.slots[t] = a.positions[t] = -1;
             continue;
         }
         // cu_new[0] = 0: the request is the last with cu_new <= t
-        const int r = upper_bound(a.cu_new, n + 1, (int)t) - 1;
-        const int grow = a.cu_new[r + 1] - a.cu_new[r];
-        map_token(a, (int)t, r, a.len_out[r] - grow + (int)t - a.cu_new[r]);
+        const int r = upper_bound(offsets, n + 1, (int)t) - 1;
+        map_token(a, (int)t, r, a.len_out[r] - offsets[r + 1] + (int)t);
     }
 }
 
@@ -639,8 +798,8 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
 
     const uint8_t *k_lane = a.k_codes + n * D + 16 * g;
     const uint8_t *v_lane = a.v_codes + (n * 4 + g) * NT * 4;
-    uint4 kr[2][NL], vr[2][NL];
-    auto load = [&](int s) {
+    uint4 kr[2][NL], vr[2][NL], kn[2][NL], vn[2][NL];
+    auto load = [&](int s, uint4 (&kr)[2][NL], uint4 (&vr)[2][NL]) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int at = min((s - k0) / 16 + b, (k1 - 1 - k0) / 16);
@@ -652,8 +811,17 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
             }
         }
     };
+    load(min(k0 + 32 * wave, k1 - 1), kn, vn);
     for (int s = k0 + 32 * wave; s < k1; s += 32 * kAttnWaves) {
-        load(s);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                kr[b][i] = kn[b][i];
+                vr[b][i] = vn[b][i];
+            }
+        // the next step's codes are on their way while this one is worked on
+        load(min(s + 32 * kAttnWaves, k1 - 1), kn, vn);
         floatx4 sc[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -699,7 +867,7 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
         // the running maximum moves only when it is passed by 2^8: p <= 256
         if (__any(mx > m_run + 8.0f)) {
             const float m_new = fmaxf(m_run, mx);
-            const float f = m_new > -INFINITY ? exp2f(m_run - m_new) : 1.0f;
+            const float f = m_new > -INFINITY ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
             l *= f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] *= f;
@@ -712,7 +880,7 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
             const float w = lane_value(vs, (s - k0) / 16 + b);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = exp2f(sc[b][i] - m_use);
+                const float p = __builtin_amdgcn_exp2f(sc[b][i] - m_use);
                 l += p;
                 const float x = p * w;
                 const _Float16 hi = (_Float16)x;
@@ -769,29 +937,53 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
     }
 }
 
-// Joins the chunks of a (row, query head); D threads, chunks in rising order.
+// Joins the chunks of a (row, query head): a wave's lanes read the chunks'
+// maxima and sums, 64 at a time, then all their parts of the output at once.
 template <typename T, int D>
-__global__ __launch_bounds__(D) void k_paged_merge(PagedAttnArgs a) {
+__global__ __launch_bounds__(64) void k_paged_merge(PagedAttnArgs a) {
+    constexpr int V = D / 64;       // dims per lane
+    typedef float vec __attribute__((ext_vector_type(V)));
     const int head = blockIdx.x % a.n_q_heads, row = blockIdx.x / a.n_q_heads;
-    const int d = threadIdx.x;
-    T *out = (T *)a.out + (int64_t)row * a.out_stride + (int64_t)head * D + d;
+    const int lane = threadIdx.x;
+    T *out = (T *)a.out + (int64_t)row * a.out_stride + (int64_t)head * D + lane * V;
+    const int64_t part = (int64_t)blockIdx.x * a.n_chunks;
+    const float2 *ml = (const float2 *)a.part_ml + part;
+    // (of chunks that do not exist there is room, and nothing is used)
+    float2 first = ml[min(lane, a.n_chunks - 1)];
     const Span sp = row_span(a, row);
     if (sp.bad || sp.len <= 0) {
-        *out = from_f32<T>(sp.bad ? __builtin_nanf("") : 0.0f);
+        for (int i = 0; i < V; ++i) out[i] = from_f32<T>(sp.bad ? __builtin_nanf("") : 0.0f);
         return;
     }
     const int n = min(a.n_chunks, (sp.len - (sp.lo & ~31) + a.chunk - 1) / a.chunk);
-    const int64_t part = (int64_t)blockIdx.x * a.n_chunks;
-    const float *ml = a.part_ml + part * 2;
-    float m = -INFINITY;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, ml[2 * i]);
-    float sum = 0.0f, acc = 0.0f;
-    for (int i = 0; i < n; ++i) {
-        const float f = ml[2 * i] == -INFINITY ? 0.0f : exp2f(ml[2 * i] - m);
-        sum += f * ml[2 * i + 1];
-        acc += f * a.part_o[(part + i) * D + d];
+    float m = -INFINITY, sum = 0.0f;
+    vec acc = {};
+    for (int c0 = 0; c0 < n; c0 += 64) {
+        if (c0) first = ml[min(c0 + lane, n - 1)];
+        const bool on = c0 + lane < n;
+        const float m_new = fmaxf(m, wave_max(on ? first.x : -INFINITY));
+        const float before = m > -INFINITY ? exp2f(m - m_new) : 0.0f;
+        // (a maximum of -inf: nothing in the chunk, or NaN, which its sum keeps)
+        const float f = on ? first.x > -INFINITY ? exp2f(first.x - m_new) : 0.0f : 0.0f;
+        float s = on ? f * first.y : 0.0f;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+        sum = sum * before + s;
+        acc *= before;
+        m = m_new;
+        const float *o = a.part_o + (part + c0) * D + lane * V;
+        const int k = min(n - c0, 64);
+        for (int i = 0; i < k; i += 16) {
+            vec x[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = *(const vec *)(o + (int64_t)min(i + j, k - 1) * D);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (i + j < k) acc += lane_value(f, i + j) * x[j];
+        }
     }
-    *out = from_f32<T>(sum != 0.0f ? acc / sum : 0.0f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = from_f32<T>(sum != 0.0f ? acc[i] / sum : 0.0f);
 }
 
 template <typename T, int FMT, int D> hipError_t attn_launch(const PagedAttnArgs &a, hipStream_t st) {
@@ -801,7 +993,7 @@ template <typename T, int FMT, int D> hipError_t attn_launch(const PagedAttnArgs
         k_paged_attn<T, FMT, D, true><<<grid, 64 * kAttnWaves, 0, st>>>(a);
     } else {
         k_paged_attn<T, FMT, D, false><<<grid, 64 * kAttnWaves, 0, st>>>(a);
-        k_paged_merge<T, D><<<(unsigned)(a.n_rows * a.n_q_heads), D, 0, st>>>(a);
+        k_paged_merge<T, D><<<(unsigned)(a.n_rows * a.n_q_heads), 64, 0, st>>>(a);
     }
     return hipGetLastError();
 }
@@ -831,10 +1023,16 @@ template <typename F> hipError_t by_types(int dtype, int code, int head_dim, F f
 }  // namespace
 
 hipError_t launch_page_map(const MapArgs &a, hipStream_t st) {
-    if (a.max_tokens <= kMapInlineTokens) {
-        k_page_map<false><<<1, kMapThreads, 0, st>>>(a);
-    } else {
-        k_page_map<true><<<1, kMapThreads, 0, st>>>(a);
+    const bool inl = a.max_tokens <= kMapInlineTokens;
+    if (a.n_req <= 64)
+        inl ? k_page_map_small<64, false><<<1, 64, 0, st>>>(a) : k_page_map_small<64, true><<<1, 64, 0, st>>>(a);
+    else if (a.n_req <= 256)
+        inl ? k_page_map_small<256, false><<<1, 256, 0, st>>>(a) : k_page_map_small<256, true><<<1, 256, 0, st>>>(a);
+    else if (a.n_req <= 1024)
+        inl ? k_page_map_small<1024, false><<<1, 1024, 0, st>>>(a) : k_page_map_small<1024, true><<<1, 1024, 0, st>>>(a);
+    else
+        inl ? k_page_map<false><<<1, kMapThreads, 0, st>>>(a) : k_page_map<true><<<1, kMapThreads, 0, st>>>(a);
+    if (!inl) {
         const int64_t wgs = ((int64_t)a.max_tokens + 255) / 256;
         k_map_tokens<<<(unsigned)(wgs < 65536 ? wgs : 65536), 256, 0, st>>>(a);
     }

@@ -159,7 +159,7 @@ vkv_status vkv_page_map(const int32_t *len_old, const int32_t *len_new, int32_t 
     if (!page_size_ok(page_size)) return bad("%s: page size %d (16, 32, 64, 128 or 256)", what, page_size);
     if (n_pages < 1 || (int64_t)n_pages * page_size > INT32_MAX) return bad("%s: %d pages", what, n_pages);
     if (table_stride < 1 || (int64_t)table_stride * page_size > INT32_MAX) return bad("%s: table stride %d", what, table_stride);
-    if (max_tokens < 0) return bad("%s: max_tokens %d", what, max_tokens);
+    if (max_tokens < 0 || max_tokens >= 1 << 30) return bad("%s: max_tokens %d", what, max_tokens);
     for (const void *p : {(const void *)len_old, (const void *)len_new, (const void *)table, (const void *)free_pages,
                           (const void *)n_free, (const void *)n_free_out, (const void *)len_out, (const void *)cu_new,
                           (const void *)status})
