@@ -12,6 +12,7 @@
 #include <cfloat>
 
 #include "vkv_serve.h"
+#include "vkv_wave.h"
 
 namespace vkv {
 namespace {
@@ -40,27 +41,6 @@ __device__ __forceinline__ float value_of(unsigned o) {
     return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 __device__ __forceinline__ u64 key_of(float x, unsigned index) { return (u64)order_of(x) << 32 | (0xffffffffu - index); }
-
-// over the wave: rotations within rows of 16 lanes, then the rows
-template <typename F> __device__ __forceinline__ float wave_reduce(float x, F f) {
-    auto turn = [](float v, auto by) {
-        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + decltype(by)::value, 0xf, 0xf, false));
-    };
-    x = f(x, turn(x, std::integral_constant<int, 8>{}));
-    x = f(x, turn(x, std::integral_constant<int, 4>{}));
-    x = f(x, turn(x, std::integral_constant<int, 2>{}));
-    x = f(x, turn(x, std::integral_constant<int, 1>{}));
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float wave_max(float x) {
-    return wave_reduce(x, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float wave_sum(float x) {
-    return wave_reduce(x, [](float a, float b) { return a + b; });
-}
 
 // A number that n of the work group's numbers (one per thread, in LDS) reach,
 // and few more (0 where n are not above 0): bit by bit from the top, each wave

@@ -12,6 +12,7 @@
 #include <cfloat>
 
 #include "vkv_serve.h"
+#include "vkv_wave.h"
 
 namespace vkv {
 namespace {
@@ -481,12 +482,6 @@ template <int FMT> __device__ __forceinline__ unsigned rescale4(unsigned w, floa
 
 template <typename T> __device__ __forceinline__ float to_f32(T x) { return (float)x; }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
-}
-
 // Eight (or four) neighbouring values of a row, as they are stored.
 template <typename T, int N> struct Raw {
     uint4 w[(N * sizeof(T) + 15) / 16];
@@ -661,25 +656,6 @@ template <int FMT> __device__ __forceinline__ half8_t codes8(unsigned w0, unsign
     return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// the other half of a lane's 16-lane row: lane n and n ^ 8
-__device__ __forceinline__ float row_ror8(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
-}
-
-// over the four 16-lane rows of a wave
-__device__ __forceinline__ float rows_max(float x) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float rows_sum(float x) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 __device__ __forceinline__ float lane_value(float x, int lane) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
 }
@@ -699,46 +675,240 @@ __device__ __forceinline__ Span row_span(const PagedAttnArgs &a, int row) {
 
 template <typename T> __device__ __forceinline__ T from_f32(float x) { return (T)x; }
 
-constexpr int kAttnWaves = 4;
+constexpr int kAttnWaves = 4, kXcds = 8;
 
-// A work group is 4 waves on (row, kv head, up to 8 query heads, chunk of
-// keys); wave w takes the chunk's 32-key steps w, w + 4, ...
-//
-// Both products run on v_mfma_f32_16x16x32_f16, whose f16 operands hold the
-// 8-bit codes exactly.  S^T = K Q^T: 16 keys by 16 columns, and O^T = V^T P:
-// 16 dims by 16 columns.  A column is a query head in the lower 8 and the
-// same head's remainder in the upper 8: q (and p) are split as hi + lo /
-// 2048 with hi and lo in f16, 22 bits together, so the result keeps the
-// accuracy of 32-bit operands without a second product: the columns would
-// else be empty for up to 8 heads per kv head.  q is first put into [1, 2)
-// by a power of two per head.
-//
-// The rows of S^T that a lane holds (keys 4 g + i of each of the step's two
-// 16-key blocks) are the keys it supplies to the second product, so P goes
-// from one product to the next in the lane's own registers.
+// A 16-token block of codes (16 D bytes) into LDS without registers: whole
+// lines, past the caches' order (one work group reads them).  Its 16-byte
+// pieces are shuffled within each row of D bytes, piece c of row r to c ^ (r
+// over the rows of a 256-byte stretch), so that the 16 lanes that read one
+// column's pieces of 16 rows at a time meet no bank twice.
+template <int D> struct Block {
+    static constexpr int pieces = D / 16, bytes = 16 * D;
+    static __device__ __forceinline__ int shuffled(int row, int piece) { return piece ^ (row / (256 / D) & (pieces - 1)); }
+    // byte of a block that lane's part of load q is to bring
+    static __device__ __forceinline__ int source(int q, int lane) {
+        const int at = q * 64 + lane, row = at / pieces;
+        return (row * pieces + shuffled(row, at % pieces)) * 16;
+    }
+    static __device__ __forceinline__ int place(int row, int piece) { return row * D + shuffled(row, piece) * 16; }
+    static __device__ __forceinline__ void load(const uint8_t *src, uint8_t *dst, const int (&from)[D / 64]) {
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)src, 0, bytes, 0x00020000);
+#pragma unroll
+        for (int q = 0; q < D / 64; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(dst + q * 1024), 16,
+                                                     from[q], 0, 0, 2 /* non-temporal */);
+    }
+};
+
+template <int N> __device__ __forceinline__ void wait_loads() {     // at most N vector loads under way
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+}
+
+// This lane's pieces of two neighbouring blocks at k, row n, and the wait for
+// them, after which their place may be written.  Written out because the
+// compiler has each LDS read wait for every load into LDS that it cannot tell
+// apart; which loads must have arrived is counted by hand (wait_loads).
+template <int D> __device__ __forceinline__ void read_blocks(const uint8_t *k, int n, int piece0, int piece1, uint4 (&w)[2][D / 64]) {
+    const unsigned base = (unsigned)(size_t)(const __attribute__((address_space(3))) uint8_t *)k;
+    const unsigned a0 = base + Block<D>::place(n, piece0), a1 = base + Block<D>::place(n, piece1);
+    if constexpr (D == 128)
+        asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:2048\n\t"
+                     "ds_read_b128 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(w[0][0]), "=&v"(w[0][D / 64 - 1]), "=&v"(w[1][0]), "=&v"(w[1][D / 64 - 1])
+                     : "v"(a0), "v"(a1)
+                     : "memory");
+    else
+        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(w[0][0]), "=&v"(w[1][0])
+                     : "v"(a0)
+                     : "memory");
+}
+
+// A wave's state: Q's column, the output's, maximum and sum so far.
+template <int D> struct AttnState {
+    half8_t q[D / 32];
+    floatx4 o[D / 16];
+    float m, l, factor;
+};
+
+// A work group's chunk of keys [begin, hi), of which [lo, hi) count: its
+// 16-key blocks' places and scales, a lane each.
+template <int D> struct Chunk {
+    const uint8_t *k_codes, *v_codes;
+    int blk, begin, lo, hi;
+    float ks, vs;
+    int from[D / 64];
+    // the two blocks at key s (the last one again behind it) on their way to `to`
+    __device__ __forceinline__ void load(const uint8_t *codes, int s, uint8_t *to) const {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int at = min((s - begin) / 16 + b, (hi - 1 - begin) / 16);
+            Block<D>::load(codes + (int64_t)__builtin_amdgcn_readlane(blk, at) * (16 * D), to + b * Block<D>::bytes, from);
+        }
+    }
+};
+
+// The 32 keys at s, of which k and v hold the codes; once they have been read,
+// those at s_next take their places.
+template <int FMT, int D>
+__device__ __forceinline__ void attn_step(uint8_t *k, uint8_t *v, const Chunk<D> &c, int s, int s_next, AttnState<D> &st) {
+    constexpr int NL = D / 64, NT = D / 16;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int at = (s - c.begin) / 16;
+    floatx4 sc[2];
+    uint4 w[2][NL];
+    read_blocks<D>(k, n, g, 4 + g, w);
+    c.load(c.k_codes, s_next, k);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        floatx4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(w[b][i].x, w[b][i].y), st.q[2 * i], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(w[b][i].z, w[b][i].w), st.q[2 * i + 1], acc, 0, 0, 0);
+        }
+        const float f = st.factor * lane_value(c.ks, at + b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = acc[i], y = row_turn<8>(x);
+            sc[b][i] = ((n < 8 ? x : y) + (n < 8 ? y : x) * (1.0f / 2048.0f)) * f;
+        }
+    }
+    unsigned keep[2] = {~0u, ~0u};
+    const bool edge = s < c.lo || s + 32 > c.hi;
+    if (edge) {
+        // the first and the last step: keys outside the span weigh nothing,
+        // and their V codes (which may be anything) become 0
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            keep[b] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = s + 16 * b + 4 * g + i;
+                const bool in = key >= c.lo && key < c.hi;
+                sc[b][i] = in ? sc[b][i] : -INFINITY;
+                keep[b] |= in ? 255u << 8 * i : 0u;
+            }
+        }
+    }
+    float mx = sc[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i / 4][i % 4]);
+    mx = rows_max(mx);
+    // the running maximum moves only when it is passed by 2^8: p <= 256
+    if (__any(mx > st.m + 8.0f)) {
+        const float m_new = fmaxf(st.m, mx);
+        const float f = m_new > -INFINITY ? __builtin_amdgcn_exp2f(st.m - m_new) : 1.0f;
+        st.l *= f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) st.o[t] *= f;
+        st.m = m_new;
+    }
+    const float m_use = st.m > -INFINITY ? st.m : 0.0f;
+    half8_t p8;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const float w = lane_value(c.vs, at + b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(sc[b][i] - m_use);
+            st.l += p;
+            const float x = p * w;
+            const _Float16 hi16 = (_Float16)x;
+            p8[4 * b + i] = n < 8 ? hi16 : (_Float16)((x - (float)hi16) * 2048.0f);
+        }
+    }
+    wait_loads<3 * 2 * NL>();
+    read_blocks<D>(v, n, NL * g, NL * g + 1, w);
+    c.load(c.v_codes, s_next, v);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        uint4 a = w[0][i], b = w[1][i];
+        if (edge) {
+            a.x &= keep[0]; a.y &= keep[0]; a.z &= keep[0]; a.w &= keep[0];
+            b.x &= keep[1]; b.y &= keep[1]; b.z &= keep[1]; b.w &= keep[1];
+        }
+        st.o[4 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(a.x, b.x), p8, st.o[4 * i], 0, 0, 0);
+        st.o[4 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(a.y, b.y), p8, st.o[4 * i + 1], 0, 0, 0);
+        st.o[4 * i + 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(a.z, b.z), p8, st.o[4 * i + 2], 0, 0, 0);
+        st.o[4 * i + 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(a.w, b.w), p8, st.o[4 * i + 3], 0, 0, 0);
+    }
+}
+
+// All of a wave's steps: two at a time over two places for K and two for V.
+// The first two steps' codes are asked for before Q is put into its form.
+template <typename T, int FMT, int D>
+__device__ __forceinline__ void attn_steps(uint8_t *k0, uint8_t *k1, uint8_t *v0, uint8_t *v1, Chunk<D> &c, bool mine, int first,
+                                           const Raw<T, 8> (&q)[D / 32], float scale, float &vref, AttnState<D> &st) {
+    constexpr int STEP = 32 * kAttnWaves, LOADS = 2 * (D / 64), NM = D / 32;
+    const int n = threadIdx.x & 15;
+    c.load(c.k_codes, first, k0);
+    c.load(c.v_codes, first, v0);
+    c.load(c.k_codes, first + STEP, k1);
+    c.load(c.v_codes, first + STEP, v1);
+    float qmax = 0.0f;
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qmax = fmaxf(qmax, fabsf(q[m][i]));
+    qmax = rows_max(qmax);
+    const int eq = qmax > 0.0f && is_finite(qmax) ? max((int)(__float_as_uint(qmax) >> 23) - 127, -126) : 0;
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = ldexpf(q[m][i], -eq);
+            const _Float16 hi = (_Float16)x;
+            st.q[m][i] = n < 8 ? hi : (_Float16)((x - (float)hi) * 2048.0f);
+        }
+    st.factor = ldexpf(scale * kLog2e, eq);
+    // V's codes are weighted by their scale over the chunk's largest: powers
+    // of two, so nothing is rounded
+    c.vs = mine ? c.vs : 0.0f;
+    vref = wave_max(c.vs);
+    c.vs *= vref > 0.0f ? 1.0f / vref : 0.0f;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) st.o[t] = floatx4{0, 0, 0, 0};
+    st.m = -INFINITY;
+    st.l = 0.0f;
+    // (waited for here: at the loop's head a wait would take in the codes)
+    asm volatile("" : "+v"(c.ks), "+v"(c.blk));
+    for (int s = first; s < c.hi; s += 2 * STEP) {
+        wait_loads<3 * LOADS>();
+        attn_step<FMT, D>(k0, v0, c, s, s + 2 * STEP, st);
+        if (s + STEP >= c.hi) break;
+        wait_loads<3 * LOADS>();
+        attn_step<FMT, D>(k1, v1, c, s + STEP, s + 3 * STEP, st);
+    }
+}
+
 template <typename T, int FMT, int D, bool DIRECT>
 __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a) {
-    constexpr int NL = D / 64;    // 16-byte loads per lane and 16-key block, K or V
-    constexpr int NM = D / 32;    // MFMAs per 16-key block of scores
-    constexpr int NT = D / 16;    // 16-dim tiles of the output
-    __shared__ float lds_o[kAttnWaves][8][D];
+    constexpr int NM = D / 32, NT = D / 16;
+    constexpr int RING = 8 * Block<D>::bytes;       // of a wave: two steps' K, then V
+    // the waves' codes on their way, and at the end their parts of the output
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kAttnWaves * RING];
     __shared__ float lds_ml[kAttnWaves][8][2];
+    float(*lds_o)[8][D] = (float(*)[8][D])lds;
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int group = a.n_q_heads / a.n_kv_heads, tiles = (group + 7) / 8;
-    const int kvh = blockIdx.x % a.n_kv_heads;
-    const int tile = blockIdx.x / a.n_kv_heads % tiles;
-    const int row = blockIdx.x / (a.n_kv_heads * tiles);
-    const int chunk = blockIdx.y;
+    // Work group i runs on XCD i mod 8.  The heads of a (row, chunk) follow
+    // each other on one XCD: a page's heads lie side by side in memory, and
+    // their scales in one line.
+    const int per = a.n_kv_heads * tiles, turn = blockIdx.x / kXcds;
+    const int unit = turn / per * kXcds + blockIdx.x % kXcds;
+    if (unit >= a.n_rows * a.n_chunks) return;
+    const int kvh = turn % per % a.n_kv_heads, tile = turn % per / a.n_kv_heads;
+    const int row = unit % a.n_rows, chunk = unit / a.n_rows;
     const int heads = min(group - 8 * tile, 8);
     const int head0 = kvh * group + 8 * tile;
 
     const Span sp = row_span(a, row);
-    const int base = sp.lo & ~31;
-    const int k0 = base + chunk * a.chunk;
-    if (sp.bad || k0 >= sp.len) {
+    const int begin = (sp.lo & ~31) + chunk * a.chunk;
+    if (sp.bad || begin >= sp.len) {
         if (DIRECT) {
             T *out = (T *)a.out + (int64_t)row * a.out_stride + (int64_t)head0 * D;
             const float v = sp.bad ? __builtin_nanf("") : 0.0f;
@@ -746,12 +916,22 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
         }
         return;
     }
-    const int k1 = min(sp.len, k0 + a.chunk);
+    const int end = min(sp.len, begin + a.chunk);
+
+    // this lane's column of Q: dims 64 i + 16 g + 8 m + [0, 8) of MFMA 2 i + m
+    // (before the codes: loads return in order)
+    Raw<T, 8> qv[NM];
+    {
+        const int col_head = head0 + min(n & 7, heads - 1);
+        const T *q = (const T *)a.q + (int64_t)row * a.q_stride + (int64_t)col_head * D;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) qv[m].load(q + 64 * (m / 2) + 16 * g + 8 * (m % 2));
+    }
 
     // The chunk's 16-key blocks, one per lane (chunk <= 1024): index of the
     // block in the layer, and its page's scales.
-    const int kb = k0 + 16 * lane;
-    const bool mine = kb < k1;
+    const int kb = begin + 16 * lane;
+    const bool mine = kb < end;
     int id = 0;
     if (mine) id = a.table[(int64_t)row * a.table_stride + kb / a.page_size];
     const bool off = id < 0 || id >= a.n_pages;
@@ -759,154 +939,30 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
     const bool bad_page = __any(mine && off);
     const int ph = id * a.n_kv_heads + kvh;
     const int blk = ph * (a.page_size / 16) + kb % a.page_size / 16;
-    const float ks = a.k_scale[ph];
-    float vs = mine ? a.v_scale[ph] : 0.0f;
-    // V's codes are weighted by their scale over the chunk's largest: powers
-    // of two, so nothing is rounded
-    float vref = wave_max(vs);
-    vs *= vref > 0.0f ? 1.0f / vref : 0.0f;
 
-    // this lane's column of Q: dims 64 i + 16 g + 8 m + [0, 8) of MFMA 2 i + m
-    const int col_head = head0 + min(n & 7, heads - 1);
-    const T *q = (const T *)a.q + (int64_t)row * a.q_stride + (int64_t)col_head * D;
-    float qv[NM][8];
-    float qmax = 0.0f;
+    Chunk<D> c{a.k_codes, a.v_codes, blk, begin, sp.lo, end, a.k_scale[ph], a.v_scale[ph], {}};
+    asm volatile("" ::: "memory");      // (those loads before the codes)
 #pragma unroll
-    for (int m = 0; m < NM; ++m)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            qv[m][i] = to_f32(q[64 * (m / 2) + 16 * g + 8 * (m % 2) + i]);
-            qmax = fmaxf(qmax, fabsf(qv[m][i]));
-        }
-    qmax = rows_max(qmax);
-    const int eq = qmax > 0.0f && is_finite(qmax) ? max((int)(__float_as_uint(qmax) >> 23) - 127, -126) : 0;
-    half8_t qf[NM];
-#pragma unroll
-    for (int m = 0; m < NM; ++m)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = ldexpf(qv[m][i], -eq);
-            const _Float16 hi = (_Float16)x;
-            qf[m][i] = n < 8 ? hi : (_Float16)((x - (float)hi) * 2048.0f);
-        }
-    const float qfac = ldexpf(a.scale * kLog2e, eq);
+    for (int q = 0; q < D / 64; ++q) c.from[q] = Block<D>::source(q, lane);
+    uint8_t *ring = lds + wave * RING;
+    AttnState<D> st;
+    float vref;
+    attn_steps<T, FMT, D>(ring, ring + 2 * Block<D>::bytes, ring + 4 * Block<D>::bytes, ring + 6 * Block<D>::bytes, c, mine,
+                          begin + 32 * wave, qv, a.scale, vref, st);
 
-    floatx4 o[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) o[t] = floatx4{0, 0, 0, 0};
-    float m_run = -INFINITY, l = 0.0f;
-
-    const uint8_t *k_lane = a.k_codes + n * D + 16 * g;
-    const uint8_t *v_lane = a.v_codes + (n * 4 + g) * NT * 4;
-    uint4 kr[2][NL], vr[2][NL], kn[2][NL], vn[2][NL];
-    auto load = [&](int s, uint4 (&kr)[2][NL], uint4 (&vr)[2][NL]) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int at = min((s - k0) / 16 + b, (k1 - 1 - k0) / 16);
-            const int64_t byte = (int64_t)__builtin_amdgcn_readlane(blk, at) * (16 * D);
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                kr[b][i] = *(const uint4 *)(k_lane + byte + 64 * i);
-                vr[b][i] = *(const uint4 *)(v_lane + byte + 16 * i);
-            }
-        }
-    };
-    load(min(k0 + 32 * wave, k1 - 1), kn, vn);
-    for (int s = k0 + 32 * wave; s < k1; s += 32 * kAttnWaves) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                kr[b][i] = kn[b][i];
-                vr[b][i] = vn[b][i];
-            }
-        // the next step's codes are on their way while this one is worked on
-        load(min(s + 32 * kAttnWaves, k1 - 1), kn, vn);
-        floatx4 sc[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            floatx4 acc = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(kr[b][i].x, kr[b][i].y), qf[2 * i], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(kr[b][i].z, kr[b][i].w), qf[2 * i + 1], acc, 0, 0, 0);
-            }
-            const float f = qfac * lane_value(ks, (s - k0) / 16 + b);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = acc[i], y = row_ror8(x);
-                sc[b][i] = ((n < 8 ? x : y) + (n < 8 ? y : x) * (1.0f / 2048.0f)) * f;
-            }
-        }
-        if (s < sp.lo || s + 32 > k1) {
-            // the first and the last step: keys outside the span weigh
-            // nothing, and their V codes (which may be anything) become 0
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                unsigned keep = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = s + 16 * b + 4 * g + i;
-                    const bool in = key >= sp.lo && key < k1;
-                    sc[b][i] = in ? sc[b][i] : -INFINITY;
-                    keep |= in ? 255u << 8 * i : 0u;
-                }
-#pragma unroll
-                for (int i = 0; i < NL; ++i) {
-                    vr[b][i].x &= keep;
-                    vr[b][i].y &= keep;
-                    vr[b][i].z &= keep;
-                    vr[b][i].w &= keep;
-                }
-            }
-        }
-        float mx = sc[0][0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i / 4][i % 4]);
-        mx = rows_max(mx);
-        // the running maximum moves only when it is passed by 2^8: p <= 256
-        if (__any(mx > m_run + 8.0f)) {
-            const float m_new = fmaxf(m_run, mx);
-            const float f = m_new > -INFINITY ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-            l *= f;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) o[t] *= f;
-            m_run = m_new;
-        }
-        const float m_use = m_run > -INFINITY ? m_run : 0.0f;
-        half8_t p8;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const float w = lane_value(vs, (s - k0) / 16 + b);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(sc[b][i] - m_use);
-                l += p;
-                const float x = p * w;
-                const _Float16 hi = (_Float16)x;
-                p8[4 * b + i] = n < 8 ? hi : (_Float16)((x - (float)hi) * 2048.0f);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint4 va = vr[0][t / 4], vb = vr[1][t / 4];
-            const unsigned wa = t % 4 == 0 ? va.x : t % 4 == 1 ? va.y : t % 4 == 2 ? va.z : va.w;
-            const unsigned wb = t % 4 == 0 ? vb.x : t % 4 == 1 ? vb.y : t % 4 == 2 ? vb.z : vb.w;
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<FMT>(wa, wb), p8, o[t], 0, 0, 0);
-        }
-    }
-
-    // the four waves' parts meet in LDS
-    l = rows_sum(l);
+    // the four waves' parts meet in LDS, where no codes are on their way any more
+    wait_loads<0>();
+    __syncthreads();
+    const float l = rows_sum(st.l);
     if (n < 8 && g == 0) {
-        lds_ml[wave][n][0] = m_run;
+        lds_ml[wave][n][0] = st.m;
         lds_ml[wave][n][1] = l;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = o[t][i], y = row_ror8(x);
+            const float x = st.o[t][i], y = row_turn<8>(x);
             if (n < 8) lds_o[wave][n][16 * t + 4 * g + i] = (x + y * (1.0f / 2048.0f)) * vref;
         }
     __syncthreads();
@@ -918,7 +974,7 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
         float sum = 0.0f, acc = 0.0f;
 #pragma unroll
         for (int w = 0; w < kAttnWaves; ++w) {
-            const float f = lds_ml[w][h][0] > -INFINITY ? exp2f(lds_ml[w][h][0] - m) : 0.0f;
+            const float f = lds_ml[w][h][0] > -INFINITY ? __builtin_amdgcn_exp2f(lds_ml[w][h][0] - m) : 0.0f;
             sum += f * lds_ml[w][h][1];
             acc += f * lds_o[w][h][d];
         }
@@ -966,8 +1022,7 @@ __global__ __launch_bounds__(64) void k_paged_merge(PagedAttnArgs a) {
         // (a maximum of -inf: nothing in the chunk, or NaN, which its sum keeps)
         const float f = on ? first.x > -INFINITY ? exp2f(first.x - m_new) : 0.0f : 0.0f;
         float s = on ? f * first.y : 0.0f;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+        s = wave_sum(s);
         sum = sum * before + s;
         acc *= before;
         m = m_new;
@@ -988,7 +1043,8 @@ __global__ __launch_bounds__(64) void k_paged_merge(PagedAttnArgs a) {
 
 template <typename T, int FMT, int D> hipError_t attn_launch(const PagedAttnArgs &a, hipStream_t st) {
     const int tiles = (a.n_q_heads / a.n_kv_heads + 7) / 8;
-    const dim3 grid((unsigned)(a.n_rows * a.n_kv_heads * tiles), (unsigned)a.n_chunks);
+    const int64_t units = ((int64_t)a.n_rows * a.n_chunks + kXcds - 1) / kXcds * kXcds;
+    const unsigned grid = (unsigned)(units * a.n_kv_heads * tiles);
     if (a.n_chunks == 1) {
         k_paged_attn<T, FMT, D, true><<<grid, 64 * kAttnWaves, 0, st>>>(a);
     } else {

@@ -239,6 +239,8 @@ vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *
     if (vkv_status s = check_rows(what, "out", out, width, dtype, &out_stride)) return s;
     PagedAttnArgs a{};
     attn_plan(units, max_len, window, &a.chunk, &a.n_chunks);
+    // (a grid has fewer than 2^32 threads)
+    if ((units + 8 * (units / n_rows)) * a.n_chunks >= 1 << 24) return bad("%s: %d rows of up to %d tokens", what, n_rows, max_len);
     const int64_t parts = (int64_t)n_rows * n_q_heads * a.n_chunks;
     if (a.n_chunks > 1) {
         const int64_t need = attn_bytes((int64_t)n_rows * n_q_heads, a.n_chunks, pages->head_dim);
