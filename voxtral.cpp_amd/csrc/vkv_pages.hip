@@ -675,7 +675,7 @@ __device__ __forceinline__ Span row_span(const PagedAttnArgs &a, int row) {
 
 template <typename T> __device__ __forceinline__ T from_f32(float x) { return (T)x; }
 
-constexpr int kAttnWaves = 4, kXcds = 8;
+constexpr int kXcds = 8;
 
 // A 16-token block of codes (16 D bytes) into LDS without registers: whole
 // lines, past the caches' order (one work group reads them).  Its 16-byte
@@ -837,10 +837,10 @@ __device__ __forceinline__ void attn_step(uint8_t *k, uint8_t *v, const Chunk<D>
 
 // All of a wave's steps: two at a time over two places for K and two for V.
 // The first two steps' codes are asked for before Q is put into its form.
-template <typename T, int FMT, int D>
+template <typename T, int FMT, int D, int WAVES>
 __device__ __forceinline__ void attn_steps(uint8_t *k0, uint8_t *k1, uint8_t *v0, uint8_t *v1, Chunk<D> &c, bool mine, int first,
                                            const Raw<T, 8> (&q)[D / 32], float scale, float &vref, AttnState<D> &st) {
-    constexpr int STEP = 32 * kAttnWaves, LOADS = 2 * (D / 64), NM = D / 32;
+    constexpr int STEP = 32 * WAVES, LOADS = 2 * (D / 64), NM = D / 32;
     const int n = threadIdx.x & 15;
     c.load(c.k_codes, first, k0);
     c.load(c.v_codes, first, v0);
@@ -882,13 +882,13 @@ __device__ __forceinline__ void attn_steps(uint8_t *k0, uint8_t *k1, uint8_t *v0
     }
 }
 
-template <typename T, int FMT, int D, bool DIRECT>
-__global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a) {
+template <typename T, int FMT, int D, int WAVES, bool DIRECT>
+__global__ __launch_bounds__(64 * WAVES) void k_paged_attn(PagedAttnArgs a) {
     constexpr int NM = D / 32, NT = D / 16;
     constexpr int RING = 8 * Block<D>::bytes;       // of a wave: two steps' K, then V
     // the waves' codes on their way, and at the end their parts of the output
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kAttnWaves * RING];
-    __shared__ float lds_ml[kAttnWaves][8][2];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[WAVES * RING];
+    __shared__ float lds_ml[WAVES][8][2];
     float(*lds_o)[8][D] = (float(*)[8][D])lds;
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -906,18 +906,6 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
     const int heads = min(group - 8 * tile, 8);
     const int head0 = kvh * group + 8 * tile;
 
-    const Span sp = row_span(a, row);
-    const int begin = (sp.lo & ~31) + chunk * a.chunk;
-    if (sp.bad || begin >= sp.len) {
-        if (DIRECT) {
-            T *out = (T *)a.out + (int64_t)row * a.out_stride + (int64_t)head0 * D;
-            const float v = sp.bad ? __builtin_nanf("") : 0.0f;
-            for (int i = tid; i < heads * D; i += 64 * kAttnWaves) out[i] = from_f32<T>(v);
-        }
-        return;
-    }
-    const int end = min(sp.len, begin + a.chunk);
-
     // this lane's column of Q: dims 64 i + 16 g + 8 m + [0, 8) of MFMA 2 i + m
     // (before the codes: loads return in order)
     Raw<T, 8> qv[NM];
@@ -928,15 +916,30 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
         for (int m = 0; m < NM; ++m) qv[m].load(q + 64 * (m / 2) + 16 * g + 8 * (m % 2));
     }
 
-    // The chunk's 16-key blocks, one per lane (chunk <= 1024): index of the
-    // block in the layer, and its page's scales.
+    // The chunk's 16-key blocks, one per lane (chunk <= 1024): their pages.
+    // Without a window the chunk's place does not depend on the length, and
+    // the table holds max_len tokens: both are read at once.
+    auto page_at = [&](int kb) { return a.table[(int64_t)row * a.table_stride + kb / a.page_size]; };
+    int id = 0;
+    if (a.window == 0 && chunk * a.chunk + 16 * lane < a.max_len) id = page_at(chunk * a.chunk + 16 * lane);
+    const Span sp = row_span(a, row);
+    const int begin = (sp.lo & ~31) + chunk * a.chunk;
+    if (sp.bad || begin >= sp.len) {
+        if (DIRECT) {
+            T *out = (T *)a.out + (int64_t)row * a.out_stride + (int64_t)head0 * D;
+            const float v = sp.bad ? __builtin_nanf("") : 0.0f;
+            for (int i = tid; i < heads * D; i += 64 * WAVES) out[i] = from_f32<T>(v);
+        }
+        return;
+    }
+    const int end = min(sp.len, begin + a.chunk);
     const int kb = begin + 16 * lane;
     const bool mine = kb < end;
-    int id = 0;
-    if (mine) id = a.table[(int64_t)row * a.table_stride + kb / a.page_size];
+    if (a.window > 0 && mine) id = page_at(kb);
     const bool off = id < 0 || id >= a.n_pages;
-    if (off) id = 0;
+    if (off || !mine) id = 0;
     const bool bad_page = __any(mine && off);
+    // the blocks' places in the layer, and their pages' scales
     const int ph = id * a.n_kv_heads + kvh;
     const int blk = ph * (a.page_size / 16) + kb % a.page_size / 16;
 
@@ -947,10 +950,10 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
     uint8_t *ring = lds + wave * RING;
     AttnState<D> st;
     float vref;
-    attn_steps<T, FMT, D>(ring, ring + 2 * Block<D>::bytes, ring + 4 * Block<D>::bytes, ring + 6 * Block<D>::bytes, c, mine,
+    attn_steps<T, FMT, D, WAVES>(ring, ring + 2 * Block<D>::bytes, ring + 4 * Block<D>::bytes, ring + 6 * Block<D>::bytes, c, mine,
                           begin + 32 * wave, qv, a.scale, vref, st);
 
-    // the four waves' parts meet in LDS, where no codes are on their way any more
+    // the waves' parts meet in LDS, where no codes are on their way any more
     wait_loads<0>();
     __syncthreads();
     const float l = rows_sum(st.l);
@@ -966,14 +969,14 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_paged_attn(PagedAttnArgs a)
             if (n < 8) lds_o[wave][n][16 * t + 4 * g + i] = (x + y * (1.0f / 2048.0f)) * vref;
         }
     __syncthreads();
-    for (int i = tid; i < heads * D; i += 64 * kAttnWaves) {
+    for (int i = tid; i < heads * D; i += 64 * WAVES) {
         const int h = i / D, d = i % D;
         float m = lds_ml[0][h][0];
 #pragma unroll
-        for (int w = 1; w < kAttnWaves; ++w) m = fmaxf(m, lds_ml[w][h][0]);
+        for (int w = 1; w < WAVES; ++w) m = fmaxf(m, lds_ml[w][h][0]);
         float sum = 0.0f, acc = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float f = lds_ml[w][h][0] > -INFINITY ? __builtin_amdgcn_exp2f(lds_ml[w][h][0] - m) : 0.0f;
             sum += f * lds_ml[w][h][1];
             acc += f * lds_o[w][h][d];
@@ -1041,14 +1044,22 @@ __global__ __launch_bounds__(64) void k_paged_merge(PagedAttnArgs a) {
     for (int i = 0; i < V; ++i) out[i] = from_f32<T>(sum != 0.0f ? acc[i] / sum : 0.0f);
 }
 
+// Up to so many work groups (two per CU) a chunk is four waves', else two
+// waves': four work groups of two fill a CU's LDS and hide each other's starts
+// and ends (64 ragged requests of up to 8192 tokens 132 -> 120 us, 4 x 8192
+// tokens 24.6 -> 19.5 us), but where all run at once the shorter chunk of a
+// wave is faster (1 x 8192 tokens 11.5 against 12.3 us, merge included).
+constexpr int64_t kAttnFew = 512;
+
 template <typename T, int FMT, int D> hipError_t attn_launch(const PagedAttnArgs &a, hipStream_t st) {
     const int tiles = (a.n_q_heads / a.n_kv_heads + 7) / 8;
     const int64_t units = ((int64_t)a.n_rows * a.n_chunks + kXcds - 1) / kXcds * kXcds;
     const unsigned grid = (unsigned)(units * a.n_kv_heads * tiles);
+    const bool few = (int64_t)a.n_rows * a.n_chunks * a.n_kv_heads * tiles <= kAttnFew;
     if (a.n_chunks == 1) {
-        k_paged_attn<T, FMT, D, true><<<grid, 64 * kAttnWaves, 0, st>>>(a);
+        few ? k_paged_attn<T, FMT, D, 4, true><<<grid, 256, 0, st>>>(a) : k_paged_attn<T, FMT, D, 2, true><<<grid, 128, 0, st>>>(a);
     } else {
-        k_paged_attn<T, FMT, D, false><<<grid, 64 * kAttnWaves, 0, st>>>(a);
+        few ? k_paged_attn<T, FMT, D, 4, false><<<grid, 256, 0, st>>>(a) : k_paged_attn<T, FMT, D, 2, false><<<grid, 128, 0, st>>>(a);
         k_paged_merge<T, D><<<(unsigned)(a.n_rows * a.n_q_heads), 64, 0, st>>>(a);
     }
     return hipGetLastError();
