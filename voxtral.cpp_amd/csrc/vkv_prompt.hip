@@ -1,7 +1,7 @@
 // Causal attention of packed prompts on gfx950.
 //
-// Two launches.  k_prompt_pack turns each prompt's K and V, 64 keys and one kv
-// head at a time, into the operands of v_mfma_f32_32x32x16: 1 KiB pieces of
+// Two launches.  k_prompt_pack turns each prompt's K and V, a tile of 64 or 32
+// keys of one kv head at a time, into the operands of v_mfma_f32_32x32x16: 1 KiB pieces of
 // 16 bytes per lane, V transposed.  Every query tile of the prompt reads them
 // again, so the transposition, the split of f32 rows and the search for the
 // largest value are paid once per key instead of once per (key, query tile).
@@ -27,7 +27,6 @@ typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kTile = kPromptKeys;
 constexpr int kTopExp = 13;     // scaled rows have their largest magnitude in [2^13, 2^14)
 constexpr int kPExp = 6;        // p <= 2^8 is scaled to <= 2^14
 
@@ -44,6 +43,9 @@ template <> struct Operand<__bf16> {
     typedef __bf16 elem;
     static constexpr int planes = 1;
 };
+
+// keys of a tile: two tiles take half of a CU's LDS at the most
+template <typename T, int D> constexpr int tile_keys() { return prompt_keys(Operand<T>::planes, D); }
 
 template <typename E> __device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
     if constexpr (std::is_same<E, __bf16>::value)
@@ -144,17 +146,17 @@ struct TileInfo {
     __device__ int odd() const { return word >> 20; }
 };
 
-// A tile's operands: K, planes x [2 blocks of 32 keys][D/16][64 lanes] 16
-// bytes: lane (r, h) has key 32 kb + r, dims 16 m + 8 h + [0, 8).  V, planes x
-// [D/32][4 blocks of 16 keys][64 lanes]: lane (r, h) has dim 32 dt + r, keys
+// A tile's operands: K, planes x [blocks of 32 keys][D/16][64 lanes] 16 bytes:
+// lane (r, h) has key 32 kb + r, dims 16 m + 8 h + [0, 8).  V, planes x
+// [D/32][blocks of 16 keys][64 lanes]: lane (r, h) has dim 32 dt + r, keys
 // 16 u + 4 h + [0, 4) and 16 u + 8 + 4 h + [0, 4), the keys whose scores a
 // lane of half h holds.
-template <typename T, int D> constexpr int tile_bytes() { return Operand<T>::planes * 2 * kTile * D * 2; }
+template <typename T, int D> constexpr int tile_bytes() { return Operand<T>::planes * 2 * tile_keys<T, D>() * D * 2; }
 
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
     typedef typename Operand<T>::elem E;
-    constexpr int NP = Operand<T>::planes;
+    constexpr int NP = Operand<T>::planes, kTile = tile_keys<T, D>(), U = kTile / 16;
     constexpr int NS = kTile * D / 8 / 256;     // 16-byte pieces per thread, K or V
     __shared__ float vt[kTile][D];
     __shared__ float red[4][2];
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
             out[PLANE + piece] = rest8<true>(kx[s]);
         }
         out[piece] = round8<E>(kx[s]);
-        const int l = piece & 63, u = (piece >> 6) & 3, dt = piece >> 8;
+        const int l = piece & 63, u = (piece >> 6) % U, dt = (piece >> 6) / U;
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -242,17 +244,15 @@ __global__ __launch_bounds__(256) void k_prompt_pack(PromptArgs a) {
 
 constexpr int kPromptThreads = 2 * kPromptRows;
 
-constexpr int kLoadThreads = kPromptThreads / 2;    // the first four waves fetch
-
 // Half a tile (K or V) into LDS without registers; buffer loads, beside which
 // the waits for LDS reads stay counted.
 template <int BYTES> __device__ __forceinline__ void fetch(const uint8_t *src, uint8_t *dst, int wave) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)src, 0, BYTES, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < BYTES / (kLoadThreads * 16); ++i)
+    for (int i = 0; i < BYTES / (kPromptThreads * 16); ++i)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rsrc, (__attribute__((address_space(3))) void *)(dst + i * (kLoadThreads * 16) + wave * 1024), 16,
-            threadIdx.x * 16, i * (kLoadThreads * 16), 0, 0);
+            rsrc, (__attribute__((address_space(3))) void *)(dst + i * (kPromptThreads * 16) + wave * 1024), 16,
+            threadIdx.x * 16, i * (kPromptThreads * 16), 0, 0);
 }
 
 __device__ __forceinline__ void wait_for_memory() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
@@ -268,8 +268,9 @@ __device__ __forceinline__ void meet() {
 // every lane its own half of the keys; the factor of the scores; the exponent
 // that O's weights are scaled by.
 template <typename T, int D> struct Rows {
-    uint4 q[Operand<T>::planes][D / 16], p[Operand<T>::planes][4];
-    floatx16 o[D / 32], s[2];
+    static constexpr int keys = tile_keys<T, D>();
+    uint4 q[Operand<T>::planes][D / 16], p[Operand<T>::planes][keys / 16];
+    floatx16 o[D / 32], s[keys / 32];
     float factor, m, l;
     int ev_ref;
     int token, t_first, t_last;
@@ -279,14 +280,16 @@ template <typename T, int D> struct Rows {
 // S^T of the tile whose K is at k
 template <typename T, int D> __device__ __forceinline__ void scores(Rows<T, D> &r, const uint8_t *k) {
     typedef typename Operand<T>::elem E;
-    constexpr int NP = Operand<T>::planes, NM = D / 16, PLANE = kTile * D * 2;
+    constexpr int NP = Operand<T>::planes, NM = D / 16, KB = Rows<T, D>::keys / 32, PLANE = KB * 32 * D * 2;
     k += (threadIdx.x & 63) * 16;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) r.s[i >> 4][i & 15] = 0.0f;
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r.s[kb][i] = 0.0f;
 #pragma unroll
     for (int m = 0; m < NM; ++m)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < KB; ++kb) {
             const uint4 hi = *(const uint4 *)(k + (kb * NM + m) * 1024);
             r.s[kb] = mfma<E>(hi, r.q[0][m], r.s[kb]);
             if constexpr (NP == 2) {
@@ -307,42 +310,40 @@ __device__ __forceinline__ void products(const PromptArgs &a, const Prompt &p, i
                                          uint8_t *__restrict__ k_next, const uint8_t *__restrict__ v_cur,
                                          uint8_t *__restrict__ v_next, Rows<T, D> &r) {
     typedef typename Operand<T>::elem E;
-    constexpr int NP = Operand<T>::planes, NM = D / 16, ND = D / 32;
-    constexpr int HALF = tile_bytes<T, D>() / 2, PLANE = kTile * D * 2;
+    constexpr int NP = Operand<T>::planes, NM = D / 16, ND = D / 32, KEYS = Rows<T, D>::keys, U = KEYS / 16;
+    constexpr int HALF = tile_bytes<T, D>() / 2, PLANE = KEYS * D * 2;
     const int lane = threadIdx.x & 63;
     if (fetches) {
         fetch<HALF>(k_src, k_next, wave);
         fetch<HALF>(v_src, v_next, wave);
     }
     if (kt + 1 < r.first_tile || kt > r.last_tile) return;
-    __builtin_amdgcn_s_setprio(1);
     const uint8_t *v = v_cur + lane * 16;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
-            const uint4 vh = *(const uint4 *)(v + (t * 4 + u) * 1024);
+            const uint4 vh = *(const uint4 *)(v + (t * U + u) * 1024);
             r.o[t] = mfma<E>(vh, r.p[0][u], r.o[t]);
             if constexpr (NP == 2) {
                 r.o[t] = mfma<E>(vh, r.p[1][u], r.o[t]);
-                r.o[t] = mfma<E>(*(const uint4 *)(v + PLANE + (t * 4 + u) * 1024), r.p[0][u], r.o[t]);
+                r.o[t] = mfma<E>(*(const uint4 *)(v + PLANE + (t * U + u) * 1024), r.p[0][u], r.o[t]);
             }
         }
     scores(r, k_cur);
     // a few operands are read ahead of the products
-    constexpr int AHEAD = NP == 2 ? 2 : 6, PAIRS = 4 * ND + 2 * NM;
+    constexpr int AHEAD = NP == 2 ? 2 : 6, PAIRS = U * ND + KEYS / 32 * NM;
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * NP, 0);
 #pragma unroll
     for (int i = 0; i < PAIRS - AHEAD; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, NP == 2 ? 3 : 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
     }
-    __builtin_amdgcn_s_setprio(0);
     if (odd) {
         // values that are not finite, left out of the product: the rows that
         // see their key take them as they are
 #pragma unroll 1
-        for (int key = kt * kTile; key < (kt + 1) * kTile && key < p.n; ++key) {
+        for (int key = kt * KEYS; key < (kt + 1) * KEYS && key < p.n; ++key) {
             const bool in = key <= r.token && (a.window <= 0 || key > r.token - a.window);
             const T *x = (const T *)a.v + (p.start + key) * a.v_stride + head * D + 4 * (lane >> 5);
 #pragma unroll
@@ -361,29 +362,29 @@ __device__ __forceinline__ void products(const PromptArgs &a, const Prompt &p, i
 template <typename T, int D>
 __device__ __forceinline__ void weights(const PromptArgs &a, int kt, TileInfo info, Rows<T, D> &r) {
     typedef typename Operand<T>::elem E;
-    constexpr int NP = Operand<T>::planes, ND = D / 32;
+    constexpr int NP = Operand<T>::planes, ND = D / 32, KEYS = Rows<T, D>::keys, U = KEYS / 16;
     if (kt < r.first_tile || kt > r.last_tile) {
 #pragma unroll
         for (int n = 0; n < NP; ++n)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) r.p[n][u] = uint4{0, 0, 0, 0};
+            for (int u = 0; u < U; ++u) r.p[n][u] = uint4{0, 0, 0, 0};
         return;
     }
     const float f = fmaxf(NP == 2 ? ldexpf(r.factor, info.ek() - kTopExp) : r.factor, FLT_MIN);
-    const int key0 = kt * kTile;
-    if (key0 + kTile - 1 > r.t_first || (a.window > 0 && key0 <= r.t_last - a.window)) {
+    const int key0 = kt * KEYS;
+    if (key0 + KEYS - 1 > r.t_first || (a.window > 0 && key0 <= r.t_last - a.window)) {
         // keys [low, high], counted from this lane's first
         const int high = r.token - key0 - 4 * (int)((threadIdx.x & 63) >> 5);
         const int low = a.window > 0 ? high - a.window + 1 : INT32_MIN;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < KEYS / 2; ++i) {
             const int j = 32 * (i >> 4) + 8 * (i >> 2 & 3) + (i & 3);
             r.s[i >> 4][i & 15] = j <= high && j >= low ? r.s[i >> 4][i & 15] : -INFINITY;
         }
     }
     float mx = r.s[0][0];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, r.s[i >> 4][i & 15]);
+    for (int i = 1; i < KEYS / 2; ++i) mx = fmaxf(mx, r.s[i >> 4][i & 15]);
     mx = halves_max(mx) * f;
     // the running maximum moves only when it is passed by 2^8
     if (__any(mx > r.m + 8.0f)) {
@@ -407,7 +408,7 @@ __device__ __forceinline__ void weights(const PromptArgs &a, int kt, TileInfo in
     }
     const float m_use = r.m > -INFINITY ? -r.m : 0.0f;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -420,26 +421,25 @@ __device__ __forceinline__ void weights(const PromptArgs &a, int kt, TileInfo in
     }
 }
 
-// A work group: 8 waves on 256 rows of one (prompt, kv head), a row being
+// A work group: 4 waves on 128 rows of one (prompt, kv head), a row being
 // (token, query head of the kv head), so the heads that share K and V read one
 // copy of them in LDS.  Wave w owns rows 32 w + [0, 32) as the columns of S^T =
 // K Q^T and O^T = V^T P^T; a lane's scores are the keys it supplies to the
 // second product, so P stays in its registers.
 //
 // The products of a tile and the softmax of a tile take about as long, on
-// units that can work at the same time, but waves that meet at every tile do
-// them at the same time and the units take turns.  So the second four waves
-// (one of the two on each SIMD) run half a tile behind the first: while one
-// wave of a SIMD multiplies, the other exponentiates.  Operands of tile kt's
-// turn (its V, the K of tile kt + 1) are in LDS for both halves of the turn;
-// those of the next come in meanwhile, by the first four waves.
+// units that can work at the same time: the registers and the LDS of a work
+// group leave room for a second one on the CU, and each SIMD's two waves, of
+// two work groups that never wait for each other, fill each other's gaps.
+// Operands of tile kt's turn (its V, the K of tile kt + 1) are in LDS at its
+// start; those of the next come in meanwhile.
 template <typename T, int D>
 __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_prompt_attn(PromptArgs a) {
     typedef typename Operand<T>::elem E;
     constexpr int NP = Operand<T>::planes;
-    constexpr int NM = D / 16, ND = D / 32;
+    constexpr int NM = D / 16, ND = D / 32, KEYS = Rows<T, D>::keys;
     constexpr int BYTES = tile_bytes<T, D>(), HALF = BYTES / 2;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // K, K, V, V
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BYTES];   // K, K, V, V
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -455,7 +455,6 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     const unsigned row0 = (unsigned)p.local * kPromptRows;
     if (row0 >= rows) return;
 
-    const bool ahead = wave < 4;
     const unsigned wrow = row0 + 32 * wave;
     const unsigned row = wrow + (lane & 31), row_in = min(row, rows - 1);
     Rows<T, D> r;
@@ -463,40 +462,38 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     const int hq = (int)(row_in - (unsigned)r.token * (unsigned)group);
     r.t_first = __builtin_amdgcn_readlane(r.token, 0);
     r.t_last = __builtin_amdgcn_readlane(r.token, 31);
-    r.first_tile = a.window > 0 && r.t_first >= a.window ? (r.t_first - a.window + 1) / kTile : 0;
-    r.last_tile = wrow < rows ? r.t_last / kTile : -2;      // a wave without rows sees no key
+    r.first_tile = a.window > 0 && r.t_first >= a.window ? (r.t_first - a.window + 1) / KEYS : 0;
+    r.last_tile = wrow < rows ? r.t_last / KEYS : -2;      // a wave without rows sees no key
     const int wg_first = (int)(row0 / (unsigned)group);
     const int wg_last = (int)(min(row0 + kPromptRows, rows) - 1) / group;
-    const int kt0 = a.window > 0 && wg_first >= a.window ? (wg_first - a.window + 1) / kTile : 0;
-    const int kt1 = wg_last / kTile;
-    const int64_t tile0 = (int64_t)head * a.n_tiles + p.start / kTile + p.seq;
+    const int kt0 = a.window > 0 && wg_first >= a.window ? (wg_first - a.window + 1) / KEYS : 0;
+    const int kt1 = wg_last / KEYS;
+    const int64_t tile0 = (int64_t)head * a.n_tiles + p.start / KEYS + p.seq;
     const uint8_t *data = a.data + tile0 * BYTES;
-    if (ahead) {
-        // K of the first tile where the turn before the first has it, then the first turn's operands
-        fetch<HALF>(data + (int64_t)kt0 * BYTES, lds + HALF, wave);
-        fetch<HALF>(data + (int64_t)min(kt0 + 1, kt1) * BYTES, lds, wave);
-        fetch<HALF>(data + (int64_t)kt0 * BYTES + HALF, lds + 2 * HALF, wave);
-    }
+    // this lane's column of Q: dims 16 m + 8 half + [0, 8)
+    float x[NM][8];
+    const T *q = (const T *)a.q + (p.start + r.token) * a.q_stride + (head * group + hq) * D + 8 * half;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) load8(q + 16 * m, x[m]);
     // the words of 64 tiles, a lane each: a load for every tile would have the
     // waits for it cover the operands that are on their way
     auto tile_words = [&](int kt) { return a.info[tile0 + min(kt + lane, kt1)]; };
     int words = tile_words(kt0);
+    // K of the first tile where the turn before the first has it, then the first turn's operands
+    fetch<HALF>(data + (int64_t)kt0 * BYTES, lds + HALF, wave);
+    fetch<HALF>(data + (int64_t)min(kt0 + 1, kt1) * BYTES, lds, wave);
+    fetch<HALF>(data + (int64_t)kt0 * BYTES + HALF, lds + 2 * HALF, wave);
 
-    // this lane's column of Q: dims 16 m + 8 half + [0, 8)
     r.factor = fabsf(a.scale) * kLog2e;
     {
-        const T *q = (const T *)a.q + (p.start + r.token) * a.q_stride + (head * group + hq) * D + 8 * half;
-        float x[NM][8];
         float qmax = 0.0f;
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            load8(q + 16 * m, x[m]);
+        for (int m = 0; m < NM; ++m)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (NP == 2) qmax = fmaxf(qmax, finite_abs(x[m][i]));
                 if (a.scale < 0.0f) x[m][i] = -x[m][i];
             }
-        }
         if constexpr (NP == 2) {
             const int e = exponent(halves_max(qmax));
             r.factor = ldexpf(r.factor, e - kTopExp);
@@ -520,19 +517,15 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
 
     wait_for_memory();
     meet();
-    if (!ahead) meet();
     scores(r, lds + HALF);
-    meet();
     TileInfo info{__builtin_amdgcn_readlane(words, 0)};
     weights(a, kt0, info, r);
     meet();
     for (int kt = kt0; kt <= kt1; ++kt) {
         const int cur = ((kt - kt0) & 1) * HALF, next = HALF - cur;
-        products<T, D>(a, p, head, kt, info.odd(), ahead && kt < kt1, wave,
-                       data + (int64_t)min(kt + 2, kt1) * BYTES,
+        products<T, D>(a, p, head, kt, info.odd(), kt < kt1, wave, data + (int64_t)min(kt + 2, kt1) * BYTES,
                        data + (int64_t)(kt + 1) * BYTES + HALF, lds + cur, lds + next, lds + 2 * HALF + cur,
                        lds + 2 * HALF + next, r);
-        meet();
         if (kt < kt1) {
             if (((kt + 1 - kt0) & 63) == 0) {
                 words = tile_words(kt + 1);
@@ -540,11 +533,10 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
             }
             info.word = __builtin_amdgcn_readlane(words, (kt + 1 - kt0) & 63);
             weights(a, kt + 1, info, r);
+            wait_for_memory();
+            meet();
         }
-        if (ahead) wait_for_memory();
-        meet();
     }
-    if (ahead) meet();
 
     const float l = halves_sum(r.l);
     if (row < rows) {
@@ -567,14 +559,8 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
 }
 
 template <typename T, int D> hipError_t prompt_launch(const PromptArgs &a, hipStream_t st) {
-    constexpr int lds = 2 * tile_bytes<T, D>();
-    auto *attn = k_prompt_attn<T, D>;
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void *)attn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) return e;
-    }
     k_prompt_pack<T, D><<<dim3((unsigned)a.n_tiles, (unsigned)a.n_kv_heads), 256, 0, st>>>(a);
-    attn<<<(unsigned)(a.n_slots * a.n_kv_heads), kPromptThreads, lds, st>>>(a);
+    k_prompt_attn<T, D><<<(unsigned)(a.n_slots * a.n_kv_heads), kPromptThreads, 0, st>>>(a);
     return hipGetLastError();
 }
 

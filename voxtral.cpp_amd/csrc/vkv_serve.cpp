@@ -135,13 +135,12 @@ int64_t attn_chunks_most(int64_t units, int32_t max_len) {
 
 int64_t attn_bytes(int64_t rows_heads, int64_t chunks, int32_t head_dim) { return rows_heads * chunks * (head_dim + 2) * 4; }
 
-int64_t prompt_tiles(int32_t n_seq, int32_t n_tokens) { return (int64_t)n_tokens / kPromptKeys + n_seq; }
+int prompt_planes(int32_t dtype) { return dtype == VKV_DTYPE_F32 ? 2 : 1; }
+int64_t prompt_tiles(int32_t n_seq, int32_t n_tokens, int keys) { return (int64_t)n_tokens / keys + n_seq; }
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
-int64_t prompt_info_bytes(int32_t n_seq, int32_t n_tokens, int32_t n_kv_heads) {
-    return round256(prompt_tiles(n_seq, n_tokens) * n_kv_heads * 4);
-}
+int64_t prompt_info_bytes(int64_t tiles, int32_t n_kv_heads) { return round256(tiles * n_kv_heads * 4); }
 
 // (maximum, sum, weighted sum) of each wave
 int64_t logprobs_stats_bytes(int64_t n_rows, int64_t chunks) { return n_rows * chunks * 4 * 16; }
@@ -279,9 +278,9 @@ size_t vkv_prompt_attn_workspace(int32_t dtype, int32_t n_seq, int32_t n_tokens,
     if (!elem_bytes(dtype) || n_seq < 0 || n_tokens < 0 || n_kv_heads < 1 || n_kv_heads > 4096 ||
         (head_dim != 64 && head_dim != 128))
         return 0;
-    const int64_t planes = dtype == VKV_DTYPE_F32 ? 2 : 1;
-    return (size_t)(prompt_info_bytes(n_seq, n_tokens, n_kv_heads) +
-                    prompt_tiles(n_seq, n_tokens) * n_kv_heads * planes * 2 * kPromptKeys * head_dim * 2);
+    const int planes = prompt_planes(dtype), keys = prompt_keys(planes, head_dim);
+    const int64_t tiles = prompt_tiles(n_seq, n_tokens, keys);
+    return (size_t)(prompt_info_bytes(tiles, n_kv_heads) + tiles * n_kv_heads * planes * 2 * keys * head_dim * 2);
 }
 
 vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
@@ -295,7 +294,7 @@ vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const
     if (n_seq < 0 || n_tokens < 0 || window < 0) return bad("%s: %d prompts of %d tokens, window %d", what, n_seq, n_tokens, window);
     if (!std::isfinite(scale)) return bad("%s: scale", what);
     PromptArgs a{};
-    a.n_tiles = prompt_tiles(n_seq, n_tokens);
+    a.n_tiles = prompt_tiles(n_seq, n_tokens, prompt_keys(prompt_planes(dtype), head_dim));
     a.n_slots = (int64_t)n_tokens * (n_q_heads / n_kv_heads) / kPromptRows + n_seq;
     if (a.n_tiles >= 1 << 24 || a.n_slots * n_kv_heads >= 1 << 23) return bad("%s: %d prompts of %d tokens", what, n_seq, n_tokens);
     if (n_seq == 0 || n_tokens == 0) return host_ok();
@@ -324,7 +323,7 @@ vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const
     a.window = window;
     a.scale = scale;
     a.info = (int32_t *)workspace;
-    a.data = (uint8_t *)workspace + prompt_info_bytes(n_seq, n_tokens, n_kv_heads);
+    a.data = (uint8_t *)workspace + prompt_info_bytes(a.n_tiles, n_kv_heads);
     StreamDevice on(as_stream(hip_stream));
     const hipError_t e = launch_prompt_attn(dtype, head_dim, a, as_stream(hip_stream));
     if (e != hipSuccess) return host_hip_fail(e, "prompt attention launch");

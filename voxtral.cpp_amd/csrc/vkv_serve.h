@@ -64,8 +64,9 @@ struct PagedAttnArgs {
 hipError_t launch_paged_attn(int dtype, int code, int head_dim, const PagedAttnArgs &a, hipStream_t st);
 
 // Causal attention of packed prompts (vkv_prompt.hip).
-constexpr int kPromptKeys = 64;     // keys per tile
-constexpr int kPromptRows = 256;    // (token, query head of a kv head) rows per work group
+constexpr int kPromptRows = 128;    // (token, query head of a kv head) rows per work group
+// Keys per tile: of K and V, `planes` 16-bit planes each, two tiles take 64 KiB
+constexpr int prompt_keys(int planes, int head_dim) { return planes * head_dim <= 128 ? 64 : 32; }
 
 struct PromptArgs {
     const void *q, *k, *v;
