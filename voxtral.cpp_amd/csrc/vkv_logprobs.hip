@@ -21,10 +21,17 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 256;
 // Pieces: 2 blocks per thread where that makes few work groups (a row or a
-// few: the time is latency), else 32 elements per thread, as many pieces per
-// work group as leave kManyGroups of them.
+// few: the time is latency) whose lists k_logprobs_join takes in one turn (a
+// row in f32, n_top 20: 12.1 us, 16.0 with 64 work groups), else 32 elements per thread, as many pieces per
+// work group as leave kManyGroups of them, which run at the same time (rows of
+// 131072 logits in bf16, n_top 20, both launches: 251 rows 23.4 us, 29.1 with
+// twice the work groups, 29.1 with 3/4; 512 rows 32.4 us, 35.7 where a work
+// group takes 4 pieces at the most, 32.5 where it takes 16).
 constexpr int kBlocksFew = 2;
 constexpr int64_t kFewGroups = 1024, kManyGroups = 1024, kTurnsMost = 8;
+// A chunk that may list more elements than this looks for its limit twice (251
+// rows as above 25.4 -> 23.4 us; n_top 5, where it lists 20, 21.1 -> 22.1 us).
+constexpr int kFewKeys = 48;
 constexpr int kWaves = kThreads / 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
@@ -42,23 +49,27 @@ __device__ __forceinline__ float value_of(unsigned o) {
 }
 __device__ __forceinline__ u64 key_of(float x, unsigned index) { return (u64)order_of(x) << 32 | (0xffffffffu - index); }
 
-// A number that n of the work group's numbers (one per thread, in LDS) reach,
-// and few more (0 where n are not above 0): bit by bit from the top, each wave
-// for itself.
-template <typename N> __device__ __forceinline__ N nth_of_group(const N *x, int n) {
-    N mine[kWaves];
+// A number that n of the work group's numbers (one per thread) reach, and few
+// more (0 where n are not above 0): bit by bit from the top.  One wave looks
+// for it: the steps are the scalar unit's, which all waves of a CU share.
+struct Search {
+    unsigned x[kThreads], found;
+};
+__device__ __forceinline__ void search_nth(Search &at, int n) {
+    if (threadIdx.x >= 64) return;
+    unsigned mine[kWaves];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mine[w] = x[w * 64 + (threadIdx.x & 63)];
-    N t = 0;
-    for (int bit = 8 * (int)sizeof(N) - 1; bit >= 0; --bit) {
-        const N up = t | (N)1 << bit;
+    for (int w = 0; w < kWaves; ++w) mine[w] = at.x[w * 64 + threadIdx.x];
+    unsigned t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned up = t | 1u << bit;
         int c = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) c += __popcll(__ballot(mine[w] >= up));
         if (c >= n) t = up;
         if (c >= n && c <= n + n / 4) break;
     }
-    return t;
+    if (threadIdx.x == 0) at.found = t;
 }
 
 // Keys of a few elements, a piece of the list for each wave; a few words
@@ -79,6 +90,13 @@ template <typename Take, typename Key> __device__ __forceinline__ void put(List 
     if (take && at < kPiece) list.key[threadIdx.x >> 6][at] = key();
     kept += __popcll(on);
 }
+
+// Blocks with elements that are not below a limit, a piece for each wave.
+constexpr int kHot = 128;
+struct Hot {
+    uint4 block[kWaves][kHot];
+    int first[kWaves][kHot];
+};
 
 // The list's n largest in falling order at out[0, n), 0 where there are fewer;
 // its keys are distinct.  A barrier is between the list's writing and this.
@@ -136,16 +154,18 @@ template <typename T> __device__ __noinline__ void pick(const T *x, int64_t from
 //
 // A value that n of the 256 threads' maxima reach is reached by n elements at
 // least, so nothing below it is among the n largest.  Found once, in the first
-// piece, it is the limit for all: what is not below it, a few more than n
-// elements per piece as a rule, goes to a list that is ranked by counting.
+// piece, by one wave while the others sum, it is the limit for all.  The blocks with elements that are not below
+// it, a few more than n per piece as a rule, are set aside whole, one test for
+// a block; at the end their elements go to a list that is ranked by counting.
 template <typename T, int BLOCKS>
 __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
     constexpr int EB = 16 / (int)sizeof(T);     // elements of a block
     constexpr int PER = BLOCKS * EB;            // of a thread and piece
     constexpr int PIECE = kThreads * PER;
     __shared__ List list;
+    __shared__ Hot hot;
+    __shared__ Search search;
     __shared__ u64 wave_best[kWaves];
-    __shared__ unsigned best[kThreads];
     __shared__ int wave_odd[kWaves];
     const int tid = threadIdx.x, chunk = blockIdx.x, row = blockIdx.y;
     const T *x = (const T *)a.logits + (int64_t)row * a.row_stride;
@@ -163,8 +183,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
     };
     uint4 next[BLOCKS];
     load(chunk0, next);
-    float m = -INFINITY, s = 0.0f, t = 0.0f, limit = -INFINITY;
-    int kept = 0;
+    float m = -INFINITY, s = 0.0f, t = 0.0f, limit = -INFINITY, largest = -INFINITY;
+    int kept = 0, set_aside = 0;
     for (int piece = chunk0; piece < end; piece += PIECE) {
         float v[PER];
 #pragma unroll
@@ -189,6 +209,14 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
 #pragma unroll
             for (int i = 1; i < EB; ++i) of_block[b] = fmaxf(of_block[b], v[b * EB + i]);
             mine = fmaxf(mine, of_block[b]);
+        }
+        largest = fmaxf(largest, mine);
+        const bool looks = a.n_top && !(limit > -INFINITY);
+        if (looks) {
+            __syncthreads();        // (the value before is read)
+            search.x[tid] = order_of(mine);
+            __syncthreads();
+            search_nth(search, a.n_top);
         }
         const float m_new = fmaxf(m, wave_max(mine));
         const float ref = m_new > -INFINITY ? m_new : 0.0f;
@@ -225,20 +253,26 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
         s = fmaf(s1, lack, s);
         t = fmaf(t1, lack, t);          // in log2 units
         if (a.n_top == 0) continue;
-        if (!(limit > -INFINITY)) {
+        if (looks) {
             __syncthreads();
-            best[tid] = order_of(mine);
-            __syncthreads();
-            limit = value_of(nth_of_group(best, a.n_top));
+            limit = value_of(search.found);
         }
-        auto at = [&](int i) { return piece + ((i / EB) * kThreads + tid) * EB + i % EB; };
         if (limit > -INFINITY) {
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b)
-                if (__any(of_block[b] >= limit))
+            for (int b = 0; b < BLOCKS; ++b) {
+                const bool take = of_block[b] >= limit;
+                const u64 on = __ballot(take);
+                if (on == 0) continue;
+                const int at = set_aside + __builtin_amdgcn_mbcnt_hi((unsigned)(on >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)on, 0));
+                if (take && at < kHot) {
+                    T y[EB] __attribute__((aligned(16)));
 #pragma unroll
-                    for (int i = b * EB; i < (b + 1) * EB; ++i)
-                        put(list, kept, v[i] >= limit, [&] { return key_of(v[i], (unsigned)at(i)); });
+                    for (int i = 0; i < EB; ++i) y[i] = (T)v[b * EB + i];
+                    hot.block[tid >> 6][at] = *(const uint4 *)y;
+                    hot.first[tid >> 6][at] = piece + (b * kThreads + tid) * EB;
+                }
+                set_aside += __popcll(on);
+            }
         } else {
             // fewer than n above -inf: they, and the chunk's first n for those of -inf that rank
 #pragma unroll 1
@@ -253,10 +287,29 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
     }
     s = wave_sum(s);
     t = wave_sum(t);
+    if (limit > -INFINITY && a.turns * a.n_top > kFewKeys) {
+        // the limit again, from all pieces: a list of few is ranked sooner
+        __syncthreads();
+        search.x[tid] = order_of(largest);
+        __syncthreads();
+        search_nth(search, a.n_top);
+        __syncthreads();
+        limit = fmaxf(limit, value_of(search.found));
+    }
+    for (int i = tid & 63; i - (tid & 63) < min(set_aside, kHot); i += 64) {
+        const bool in = i < min(set_aside, kHot);
+        const uint4 y = hot.block[tid >> 6][min(i, kHot - 1)];
+        const int first = hot.first[tid >> 6][min(i, kHot - 1)];
+#pragma unroll
+        for (int q = 0; q < EB; ++q) {
+            const float z = (float)((const T *)&y)[q];
+            put(list, kept, in && z >= limit, [&] { return key_of(z, (unsigned)(first + q)); });
+        }
+    }
     if ((tid & 63) == 0) {
         *((float4 *)a.stats + ((int64_t)row * a.n_chunks + chunk) * kWaves + (tid >> 6)) = float4{m, s, t * kLn2, 0.0f};
         list.count[tid >> 6] = min(kept, kPiece);
-        wave_odd[tid >> 6] = s != s || kept > kPiece;   // NaN or +inf, or a full list
+        wave_odd[tid >> 6] = s != s || kept > kPiece || set_aside > kHot;   // NaN or +inf, or a full list
     }
     if (a.n_top == 0) return;
     __syncthreads();
@@ -275,7 +328,7 @@ constexpr int kJoinPer = 3;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
     __shared__ List list;
-    __shared__ u64 bests[kThreads];
+    __shared__ Search search;
     __shared__ u64 top[kLogprobsMaxTop];
     __shared__ float red[kWaves][4];
     const int tid = threadIdx.x, row = blockIdx.x;
@@ -284,10 +337,12 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
     const u64 *keys = a.keys + (int64_t)row * a.n_chunks * a.n_top;
     const int n_keys = a.n_chunks * a.n_top;
 
-    // everything the row needs is asked for at once
+    // everything the row needs is asked for at once; the waves take turns at
+    // the keys, so that few of them are shared out evenly
+    const int mine = (tid & 63) * kWaves + (tid >> 6);
     u64 k[kJoinPer];
 #pragma unroll
-    for (int i = 0; i < kJoinPer; ++i) k[i] = i * kThreads + tid < n_keys ? keys[i * kThreads + tid] : 0;
+    for (int i = 0; i < kJoinPer; ++i) k[i] = i * kThreads + mine < n_keys ? keys[i * kThreads + mine] : 0;
     const int token = a.tokens ? a.tokens[row] : -1;
     const bool is_token = token >= 0 && token < a.n_vocab;
     const float at_token = is_token ? (float)((const T *)a.logits)[row * a.row_stride + token] : 0.0f;
@@ -326,7 +381,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
         if (base)
 #pragma unroll
             for (int i = 0; i < kJoinPer; ++i) {
-                const int at = base + i * kThreads + tid;
+                const int at = base + i * kThreads + mine;
                 k[i] = at < n_keys ? keys[at] : 0;
             }
         u64 best = 0;
@@ -335,9 +390,11 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
         u64 least = 1;
         __syncthreads();
         if (n_keys > kThreads) {        // (else the list takes them all)
-            bests[tid] = best;
+            search.x[tid] = (unsigned)(best >> 32);
             __syncthreads();
-            least = max(nth_of_group(bests, a.n_top), (u64)1);
+            search_nth(search, a.n_top);
+            __syncthreads();
+            least = max((u64)search.found << 32, (u64)1);
         }
         int kept = 0;
 #pragma unroll
@@ -377,20 +434,19 @@ template <typename T> hipError_t run(const LogprobsArgs &a, int blocks, hipStrea
 
 }  // namespace
 
-LogprobsPlan logprobs_plan(int n_rows, int64_t n_vocab, int elem_bytes) {
+LogprobsPlan logprobs_plan(int n_rows, int64_t n_vocab, int elem_bytes, int n_top, bool rows_aligned) {
     // blocks of a row, wherever in a block it begins
-    const int64_t blocks = (n_vocab + 2 * (16 / elem_bytes) - 2) / (16 / elem_bytes);
+    const int64_t per = 16 / elem_bytes, blocks = (n_vocab + (rows_aligned ? 1 : 2) * (per - 1)) / per;
     LogprobsPlan p;
     const int64_t small = (blocks + kBlocksFew * kThreads - 1) / (kBlocksFew * kThreads);
-    p.blocks = n_rows * small <= kFewGroups ? kBlocksFew : elem_bytes == 4 ? 8 : 4;
+    p.blocks = n_rows * small <= kFewGroups && small * n_top <= kThreads * kJoinPer ? kBlocksFew : elem_bytes == 4 ? 8 : 4;
     const int64_t pieces = (blocks + p.blocks * kThreads - 1) / (p.blocks * kThreads);
-    p.turns = (int32_t)std::min<int64_t>(std::max<int64_t>(n_rows * pieces / kManyGroups, 1), std::min<int64_t>(pieces, kTurnsMost));
+    p.turns = (int32_t)std::min<int64_t>((n_rows * pieces + kManyGroups - 1) / kManyGroups, std::min<int64_t>(pieces, kTurnsMost));
     p.chunks = (int32_t)((pieces + p.turns - 1) / p.turns);
     return p;
 }
 
-hipError_t launch_logprobs(int dtype, const LogprobsArgs &a, hipStream_t st) {
-    const int blocks = logprobs_plan(a.n_rows, a.n_vocab, dtype == VKV_DTYPE_F32 ? 4 : 2).blocks;
+hipError_t launch_logprobs(int dtype, const LogprobsArgs &a, int blocks, hipStream_t st) {
     if (dtype == VKV_DTYPE_F16) return run<_Float16>(a, blocks, st);
     if (dtype == VKV_DTYPE_BF16) return run<__bf16>(a, blocks, st);
     return run<float>(a, blocks, st);

@@ -333,7 +333,9 @@ vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const
 size_t vkv_logprobs_workspace(int32_t n_rows, int64_t n_vocab, int32_t n_top) {
     if (n_rows < 0 || n_vocab < 1 || n_vocab > 1 << 30 || n_top < 0 || n_top > kLogprobsMaxTop) return 0;
     int64_t most = 0;
-    for (int eb : {2, 4}) most = std::max<int64_t>(most, logprobs_plan(n_rows, n_vocab, eb).chunks);
+    for (int eb : {2, 4})
+        for (bool aligned_rows : {false, true})
+            most = std::max<int64_t>(most, logprobs_plan(n_rows, n_vocab, eb, n_top, aligned_rows).chunks);
     return (size_t)(logprobs_stats_bytes(n_rows, most) + n_rows * most * n_top * 8);
 }
 
@@ -356,7 +358,7 @@ vkv_status vkv_logprobs(int32_t dtype, const void *logits, int64_t row_stride, i
             if (vkv_status s = check_ints(what, p)) return s;
     if (!aligned(tokens, 4) || !aligned(logprob, 4) || !aligned(entropy, 4))
         return bad("%s: int32 and f32 arrays must be 4-byte aligned", what);
-    const LogprobsPlan plan = logprobs_plan(n_rows, n_vocab, eb);
+    const LogprobsPlan plan = logprobs_plan(n_rows, n_vocab, eb, n_top, n_rows == 1 || row_stride * eb % 16 == 0);
     const int64_t chunks = plan.chunks;
     const int64_t stats = logprobs_stats_bytes(n_rows, chunks), need = stats + n_rows * chunks * n_top * 8;
     if ((int64_t)workspace_bytes < need) return small_ws(what, workspace_bytes, (size_t)need);
@@ -364,7 +366,7 @@ vkv_status vkv_logprobs(int32_t dtype, const void *logits, int64_t row_stride, i
     LogprobsArgs a{logits, row_stride, n_rows, (int32_t)n_vocab, n_top, plan.chunks, plan.turns, tokens, logprob, entropy,
                    top_ids, top_logprobs, (float *)workspace, (unsigned long long *)((uint8_t *)workspace + stats)};
     StreamDevice on(as_stream(hip_stream));
-    const hipError_t e = launch_logprobs(dtype, a, as_stream(hip_stream));
+    const hipError_t e = launch_logprobs(dtype, a, plan.blocks, as_stream(hip_stream));
     if (e != hipSuccess) return host_hip_fail(e, "log probabilities launch");
     return host_ok();
 }

@@ -98,11 +98,12 @@ struct LogprobsArgs {
     unsigned long long *keys;           // [row][chunk][n_top]
 };
 
-// 16-byte blocks per thread and piece, pieces per chunk, chunks per row
+// 16-byte blocks per thread and piece, pieces per chunk, chunks per row;
+// rows_aligned: every row begins at a 16-byte boundary
 struct LogprobsPlan {
     int32_t blocks, turns, chunks;
 };
-LogprobsPlan logprobs_plan(int n_rows, int64_t n_vocab, int elem_bytes);
-hipError_t launch_logprobs(int dtype, const LogprobsArgs &a, hipStream_t st);
+LogprobsPlan logprobs_plan(int n_rows, int64_t n_vocab, int elem_bytes, int n_top, bool rows_aligned);
+hipError_t launch_logprobs(int dtype, const LogprobsArgs &a, int blocks, hipStream_t st);
 
 }  // namespace vkv
