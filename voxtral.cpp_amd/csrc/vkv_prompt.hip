@@ -332,9 +332,9 @@ template <typename T, int D> __device__ __forceinline__ void scores(Rows<T, D> &
 // The matrix cores' half of a tile: O^T += V^T P^T for the tile whose weights
 // are at hand, and the scores of the next.  The next tile's operands are
 // fetched into the other places on the way: the four are restrict, or each
-// read would wait for the loads.
-template <typename T, int D>
-__device__ __forceinline__ void products(const PromptArgs &a, const Prompt &p, int head, int kt, int odd, bool fetches, int wave,
+// read would wait for the loads.  LAST: there is no next.
+template <typename T, int D, bool LAST>
+__device__ __forceinline__ void products(const PromptArgs &a, const Prompt &p, int head, int kt, int odd, int wave,
                                          const uint8_t *k_src, const uint8_t *v_src, const uint8_t *__restrict__ k_cur,
                                          uint8_t *__restrict__ k_next, const uint8_t *__restrict__ v_cur,
                                          uint8_t *__restrict__ v_next, Rows<T, D> &r) {
@@ -342,7 +342,7 @@ __device__ __forceinline__ void products(const PromptArgs &a, const Prompt &p, i
     constexpr int NP = Operand<T>::planes, NM = D / 16, ND = D / 32, KEYS = Rows<T, D>::keys, U = KEYS / 16;
     constexpr int HALF = tile_bytes<T, D>() / 2, PLANE = KEYS * D * 2;
     const int lane = threadIdx.x & 63;
-    if (fetches) {
+    if constexpr (!LAST) {
         fetch<HALF>(k_src, k_next, wave);
         fetch<HALF>(v_src, v_next, wave);
     }
@@ -359,9 +359,9 @@ __device__ __forceinline__ void products(const PromptArgs &a, const Prompt &p, i
                 r.o[t] = mfma<E>(*(const uint4 *)(v + PLANE + (t * U + u) * 1024), r.p[0][u], r.o[t]);
             }
         }
-    scores(r, k_cur);
+    if constexpr (!LAST) scores(r, k_cur);
     // a few operands are read ahead of the products
-    constexpr int AHEAD = NP == 2 ? 2 : 6, PAIRS = U * ND + KEYS / 32 * NM;
+    constexpr int AHEAD = NP == 2 ? 2 : 6, PAIRS = U * ND + (LAST ? 0 : KEYS / 32 * NM);
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * NP, 0);
 #pragma unroll
     for (int i = 0; i < PAIRS - AHEAD; ++i) {
@@ -515,28 +515,37 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     fetch<HALF>(data + (int64_t)kt0 * BYTES + HALF, lds + 2 * HALF, wave);
 
     r.factor = fabsf(a.scale) * kLog2e;
-    {
-        float qmax = 0.0f;
+    float by = a.scale < 0.0f ? -1.0f : 1.0f;
+    bool fine = true;       // the largest value's exponent is that of finite ones
+    if constexpr (NP == 2) {
+        unsigned top = 0;
 #pragma unroll
         for (int m = 0; m < NM; ++m)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (NP == 2) qmax = fmaxf(qmax, finite_abs(x[m][i]));
-                if (a.scale < 0.0f) x[m][i] = -x[m][i];
-            }
-        if constexpr (NP == 2) {
-            const int e = exponent(halves_max(qmax));
-            r.factor = ldexpf(r.factor, e - kTopExp);
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[m][i]) & 0x7fffffffu);
+        fine = !__any(top >= 0x7f800000u);
+        if (!fine) {
+            top = 0;
 #pragma unroll
-            for (int m = 0; m < NM; ++m) {
+            for (int m = 0; m < NM; ++m)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[m][i] = ldexpf(x[m][i], kTopExp - e);
-                r.q[1][m] = rest8<true>(x[m]);
-            }
+                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(finite_abs(x[m][i])));
         }
-#pragma unroll
-        for (int m = 0; m < NM; ++m) r.q[0][m] = round8<E>(x[m]);
+        const int e = exponent(halves_max(__uint_as_float(top)));
+        r.factor = ldexpf(r.factor, e - kTopExp);
+        by = ldexpf(by, kTopExp - e);
     }
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[m][i] *= by;
+        r.q[0][m] = round8<E>(x[m]);
+        if constexpr (NP == 2) r.q[1][m] = rest8<false>(x[m]);
+    }
+    if (!fine)
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+            if constexpr (NP == 2) r.q[1][m] = rest8<true>(x[m]);
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -551,22 +560,22 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     TileInfo info{__builtin_amdgcn_readlane(words, 0)};
     weights(a, kt0, info, r);
     meet();
-    for (int kt = kt0; kt <= kt1; ++kt) {
-        const int cur = ((kt - kt0) & 1) * HALF, next = HALF - cur;
-        products<T, D>(a, p, head, kt, info.odd(), kt < kt1, wave, data + (int64_t)min(kt + 2, kt1) * BYTES,
-                       data + (int64_t)(kt + 1) * BYTES + HALF, lds + cur, lds + next, lds + 2 * HALF + cur,
-                       lds + 2 * HALF + next, r);
-        if (kt < kt1) {
-            if (((kt + 1 - kt0) & 63) == 0) {
-                words = tile_words(kt + 1);
-                asm volatile("" : "+v"(words));     // waited for here, not at every tile
-            }
-            info.word = __builtin_amdgcn_readlane(words, (kt + 1 - kt0) & 63);
-            weights(a, kt + 1, info, r);
-            wait_for_memory();
-            meet();
+    int cur = 0;
+    for (int kt = kt0; kt < kt1; ++kt, cur = HALF - cur) {
+        const int next = HALF - cur;
+        products<T, D, false>(a, p, head, kt, info.odd(), wave, data + (int64_t)min(kt + 2, kt1) * BYTES,
+                              data + (int64_t)(kt + 1) * BYTES + HALF, lds + cur, lds + next, lds + 2 * HALF + cur,
+                              lds + 2 * HALF + next, r);
+        if (((kt + 1 - kt0) & 63) == 0) {
+            words = tile_words(kt + 1);
+            asm volatile("" : "+v"(words));     // waited for here, not at every tile
         }
+        info.word = __builtin_amdgcn_readlane(words, (kt + 1 - kt0) & 63);
+        weights(a, kt + 1, info, r);
+        wait_for_memory();
+        meet();
     }
+    products<T, D, true>(a, p, head, kt1, info.odd(), wave, nullptr, nullptr, nullptr, nullptr, lds + 2 * HALF + cur, nullptr, r);
 
     const float l = halves_sum(r.l);
     if (row < rows) {
