@@ -846,8 +846,9 @@ vkv_status vkv_page_map(const int32_t *len_old, const int32_t *len_new, int32_t 
  * ties to even; what is not finite becomes NaN in e4m3, and in int8 0 (NaN) or
  * the largest code of its sign.  A slot outside the pool (-1: a token of
  * another call, or padding) is skipped.  The tokens of one page must stand
- * next to each other in the call, as vkv_page_map leaves them, in any order;
- * of several rows for one slot the last counts. */
+ * next to each other in the call, as vkv_page_map leaves them, with no skipped
+ * one between them, in any order; of several rows for one slot the last
+ * counts. */
 vkv_status vkv_pages_append(const vkv_pages *pages, int32_t layer, const int32_t *slots,
                             int32_t n_tokens, int32_t dtype, const void *k, const void *v,
                             int64_t row_stride, void *hip_stream);
@@ -879,8 +880,11 @@ vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *
  * arrays hold n_tokens rows; rows behind the last prompt are not read, and
  * those of out are left as they are.  Prompts may be empty.  Keys that a row
  * does not attend to have no effect on it, whatever they hold.
- * F32 rows are multiplied as pairs of f16 (22 bits), F16 and BF16 rows as they
- * are, with the softmax weights rounded to that type; sums are 32-bit.
+ * F32 rows are multiplied as pairs of f16: 22 bits of a value that is within
+ * 2^-16 of the largest of its q row and head or, in k and v, of its kv head's
+ * 32 or 64 neighbouring keys; steps of 2^-38 of that largest below.  F16 and
+ * BF16 rows are multiplied as they are, with the softmax weights rounded to
+ * that type.  Sums are 32-bit.
  * The workspace is 256-byte aligned; its contents do not matter. */
 size_t vkv_prompt_attn_workspace(int32_t dtype, int32_t n_seq, int32_t n_tokens,
                                  int32_t n_kv_heads, int32_t head_dim);

@@ -79,6 +79,13 @@ def test_page_map_with_many_tokens_is_the_same():
         assert np.array_equal(g.cpu().numpy().reshape(-1), np.asarray(w).reshape(-1))
 
 
+@pytest.mark.parametrize("n_req,page,stride,most", [(65, 16, 9, 100), (200, 32, 4, 90), (256, 16, 8, 12), (257, 16, 3, 40),
+                                                    (4100, 16, 2, 3), (5000, 16, 3, 30)])
+def test_page_map_of_larger_batches(n_req, page, stride, most):
+    """each of the map's forms at its ends, with few and with many new tokens"""
+    test_page_map_equals_the_loops(n_req, page, stride, most)
+
+
 @pytest.mark.parametrize("what,status", [
     ("short", 1), ("short of one page", 1), ("negative old", 2), ("negative new", 2), ("beyond the table", 2), ("too many tokens", 2),
     ("stack beyond the pool", 2), ("stack below 0", 2), ("returns no page", 2), ("more returned than the stack holds", 2),
@@ -201,6 +208,33 @@ def test_append_skips_repeats_and_disorder(code):
     pool.append(i32(slots), rows_on_device(k, vkv.F32), rows_on_device(v, vkv.F32), vkv.F32)
     model.append(slots, k, v)
     same_pages(pool, model)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("page,heads,dim,run", [(16, 3, 64, 50), (32, 2, 128, 7), (64, 1, 128, 300), (128, 1, 64, 700), (256, 1, 64, 90)])
+def test_append_of_many_tokens(page, heads, dim, run, code):
+    """more tokens than have a work group each: every page is begun with its slot 0, then runs begin and end anywhere in
+    a page, twice; padding behind them"""
+    rng = np.random.default_rng(run)
+    n_pages, n = 0, 1300
+    runs = []
+    left = n
+    while left:
+        m = min(left, int(rng.integers(1, run + 1)))
+        runs.append((int(rng.integers(0, page)), m))
+        n_pages += -(-(runs[-1][0] + m) // page)
+        left -= m
+    order, slots, at = rng.permutation(n_pages), [], 0
+    for first, m in runs:
+        slots += [int(order[at + i // page]) * page + i % page for i in range(first, first + m)]
+        at += -(-(first + m) // page)
+    pool, model = Pool(code, n_pages, page, heads, dim), PoolModel(code, n_pages, page, heads, dim)
+    for put in ([p * page for p in range(n_pages)], slots[:700], slots[700:] + [-1] * 30, slots):
+        k, v = (wide_rows(rng, len(put), heads * dim, vkv.BF16) for _ in range(2))
+        k, v = (rows_on_device(x, vkv.BF16) for x in (k, v))
+        pool.append(i32(put), k, v, vkv.BF16)
+        model.append(put, as64(k), as64(v))
+        same_pages(pool, model)
 
 
 @pytest.mark.parametrize("code", CODES)

@@ -83,6 +83,31 @@ def test_prompt_attn_many_prompts():
     check([1] * 70 + [130] + [0] * 64 + [3], 2, 2, 64, vkv.F16)
 
 
+@pytest.mark.parametrize("n", [63, 64, 65])
+def test_prompt_attn_of_prompts_in_order_of_length(n):
+    """up to 64 prompts are taken by length, more in their order"""
+    rng = np.random.default_rng(n)
+    lens = list(rng.integers(0, 20, n))
+    lens[3], lens[n // 2], lens[-1] = 200, 333, 131
+    check(lens, 4, 1, 64, vkv.BF16)
+
+
+@pytest.mark.parametrize("window", [0, 2100])
+def test_prompt_attn_of_more_than_64_tiles(window):
+    check([9, 2300], 1, 1, 128, vkv.F32, window)
+
+
+def test_prompt_attn_offsets_that_count_rows_many_times():
+    """64 prompts that each claim every row: the accesses stay in the arrays, the call ends"""
+    rng = np.random.default_rng(11)
+    H, Hk, D, n = 2, 1, 64, 300
+    q, k, v = (rows_on_device(rng.standard_normal((n, h * D)), vkv.F16) for h in (H, Hk, Hk))
+    call(q, k, v, [0, n] * 32 + [0], H, Hk, D, vkv.F16)
+    torch.cuda.synchronize()
+    want = call(q, k, v, [0, n], H, Hk, D, vkv.F16)
+    assert torch.equal(call(q, k, v, [0] * 64 + [n], H, Hk, D, vkv.F16), want)
+
+
 @pytest.mark.parametrize("gain,scale", [(300.0, None), (1e-30, None), (1.0, -0.1), (1.0, 0.0), (1e30, 1e-31)])
 def test_prompt_attn_of_scores_far_apart(gain, scale):
     check([130, 70], 4, 2, 128, vkv.F32, gain=gain, scale=scale)
@@ -216,6 +241,50 @@ def test_logprobs_ties_go_to_the_lowest_id(dtype):
               np.tile(np.arange(n) % 40 / 4, (2, 1)), np.sort(rng.standard_normal((2, n)), 1),
               -np.sort(rng.standard_normal((2, n)), 1), np.where(rng.random((2, n)) < 0.5, 0.0, -0.0)):
         check_logprobs(x, [0, n - 1], 32, dtype)
+
+
+@pytest.mark.parametrize("dtype", [vkv.F32, vkv.BF16])
+def test_logprobs_of_many_rows_of_every_kind(dtype):
+    """several pieces to a work group: values that rise, so that the first piece's limit keeps nothing out, or fall;
+    many equal ones; few that are not -inf, in the first piece or behind it; NaN and +inf"""
+    rng = np.random.default_rng(12)
+    n, v, top = 200, 40001, 32
+    x = rng.standard_normal((n, v)) * 3
+    x[:20] = np.sort(x[:20], 1)
+    x[20:40] = -np.sort(-x[20:40], 1)
+    x[40:60] = rng.integers(0, 3, (20, v))
+    for r in range(60, 80):
+        x[r, rng.permutation(v)[:v - 1 - r % 40]] = -np.inf
+    x[80:85, :39990] = -np.inf
+    x[85:90, 11:] = -np.inf
+    x[90:95] = -np.inf
+    x[95:100, 0] = 1e6 if dtype == vkv.F32 else 1e4
+    tokens = rng.integers(0, v, n)
+    x[100, 39999], x[101, 3], x[102, 20000] = np.nan, np.inf, np.nan
+    got = logprobs(rows_on_device(x, dtype), tokens, top, dtype)
+    x = as64(rows_on_device(x, dtype))
+    rows = np.r_[0:90, 95:100, 103:n]
+    want = logprobs_reference(x[rows], tokens[rows], top)
+    assert np.array_equal(got[2][rows], want[2])
+    rel = (24 + 32 + np.log2(v)) * 2.0 ** -24
+    with np.errstate(invalid="ignore"):
+        for g, w in ((got[0][rows], want[0]), (got[3][rows], want[3])):
+            assert ((np.abs(g - w) <= rel + 3 * 2.0 ** -24 * np.abs(w)) | (g == w)).all()
+    assert (np.abs(got[1][rows] - want[1]) <= rel * (2 + 2 * np.log(v))).all()
+    for r in range(90, 95):
+        assert got[0][r] == -np.inf and got[1][r] == 0 and got[2][r].tolist() == list(range(top)) and (got[3][r] == -np.inf).all()
+    for r, first in ((100, 39999), (101, 3), (102, 20000)):
+        assert np.isnan(got[0][r]) and np.isnan(got[1][r]) and np.isnan(got[3][r]).all() and got[2][r, 0] == first
+
+
+@pytest.mark.parametrize("vocab,rows", [(5000, 5), (20001, 300)])
+def test_logprobs_of_large_logits(vocab, rows):
+    """spread over, or all near, magnitudes at which a unit is many, few and none of f32's steps"""
+    rng = np.random.default_rng(13)
+    x = rng.standard_normal((rows, vocab)) * np.array([1e2, 1e4, 1e6, 1e9, 1e30])[np.arange(rows) % 5, None]
+    check_logprobs(x, rng.integers(0, vocab, rows), 3, vkv.F32)
+    x = rng.standard_normal((rows, vocab)) + np.array([1e2, -1e4, 1e6, -3e7, 1e10])[np.arange(rows) % 5, None]
+    check_logprobs(x, rng.integers(0, vocab, rows), 3, vkv.F32)
 
 
 def test_logprobs_masked_rows():
@@ -408,6 +477,34 @@ def test_a_step_in_a_graph():
             assert torch.equal(a.nan_to_num(), b.nan_to_num()), (n, name)
         for name in ("table", "free", "n_free", "lens", "cu", "slots", "positions", "status"):
             assert torch.equal(getattr(eager.map, name), getattr(s.map, name)), (n, name)
+        for a, b in zip(eager.pool.codes + eager.pool.scale, s.pool.codes + s.pool.scale):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_prompts_in_a_graph():
+    """admitting prompts, captured once, replayed with other prompts and other work between the replays"""
+    eager, s = server(8), server(8)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        s.admit()           # of no prompt: warms up, changes nothing
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.admit()
+    for lens in ([20, 3, 40, 1], [0, 0, 0, 120], [128, 0, 0, 0], [1, 1, 1, 1], [64, 0, 56, 0]):
+        for x in (eager, s):
+            x.out.fill_(7.0)
+            x.new.zero_()
+            x.map.call(x.new)           # all pages back
+            x.new.copy_(i32(lens))
+            x.v.add_(0.5)
+        eager.admit()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager.out, s.out) and eager.map.status.item() == (2 if sum(lens) > 120 else 0)
+        used = sum(lens) if sum(lens) <= 120 else 0
+        assert (s.out[used:] == 7.0).all() and not (used and (s.out[:used] == 7.0).all())
         for a, b in zip(eager.pool.codes + eager.pool.scale, s.pool.codes + s.pool.scale):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 

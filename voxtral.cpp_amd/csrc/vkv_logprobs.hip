@@ -237,9 +237,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
             s1 += e;
             t1 = fmaf(e, d, t1);
         }
-        if (__any(!(fabsf(t1) <= FLT_MAX))) {
-            // a logit of -inf (0 times the logarithm of 0 is 0), or a c beyond
-            // the range: d from the difference
+        if (__any(!(fabsf(t1) <= FLT_MAX && fabsf(lack) <= 1.0f))) {
+            // a logit of -inf (0 times the logarithm of 0 is 0), or one so
+            // large that c lacks whole powers of two: d from the difference
             lack = s1 = t1 = 0.0f;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
             }
         }
         t1 = fmaf(-lack, s1, t1);
-        lack = fmaf(-lack, kLn2, 1.0f);
+        lack = __builtin_amdgcn_exp2f(-lack);
         s = fmaf(s1, lack, s);
         t = fmaf(t1, lack, t);          // in log2 units
         if (a.n_top == 0) continue;

@@ -159,7 +159,9 @@ __device__ __forceinline__ bool find_longest(const PromptArgs &a, int at, int mu
     const int nth = at - from(low + 1);
     const unsigned long long there = __ballot(tiles > low);
     const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(there >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)there, 0));
-    p.seq = __ffsll(__ballot(tiles > low && before == nth)) - 1;
+    const unsigned long long it = __ballot(tiles > low && before == nth);
+    if (it == 0) return false;      // (offsets that are none, with more tiles than can be counted)
+    p.seq = __ffsll(it) - 1;
     p.start = __builtin_amdgcn_readlane(start, p.seq);
     p.n = __builtin_amdgcn_readlane(n, p.seq);
     p.local = low;
