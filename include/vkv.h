@@ -879,7 +879,8 @@ vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *
  * of a prompt attends to its tokens (t - window, t] (window 0: [0, t]).  The
  * arrays hold n_tokens rows; rows behind the last prompt are not read, and
  * those of out are left as they are.  Prompts may be empty.  Keys that a row
- * does not attend to have no effect on it, whatever they hold.
+ * does not attend to have no effect on it, NaN and infinities among them (in
+ * F32 but for the bits below).
  * F32 rows are multiplied as pairs of f16: 22 bits of a value that is within
  * 2^-16 of the largest of its q row and head or, in k and v, of its kv head's
  * 32 or 64 neighbouring keys; steps of 2^-38 of that largest below.  F16 and

@@ -113,6 +113,25 @@ def test_prompt_attn_of_scores_far_apart(gain, scale):
     check([130, 70], 4, 2, 128, vkv.F32, gain=gain, scale=scale)
 
 
+@pytest.mark.parametrize("dtype", [vkv.F32, vkv.F16, vkv.BF16])
+@pytest.mark.parametrize("scale", [1e6, -1e8, 1e20])
+def test_prompt_attn_of_scores_beyond_their_own_steps(dtype, scale):
+    """scores so large that neighbouring f32 values are several units apart: a row takes its largest key alone (no two
+    of these keys are nearly as large), and equal keys share it"""
+    rng = np.random.default_rng(14)
+    n, D = 150, 64
+    q = np.ones((n, D))
+    size = rng.permutation(n)               # q . k = 64 * size: exact in every type
+    k = np.repeat(size[:, None], D, 1).astype(float)
+    k[100:110] = k[99] + 1000
+    v = rng.integers(-8, 9, (n, D)).astype(float)
+    got = as64(call(*(rows_on_device(x, dtype) for x in (q, k, v)), [0, n], 1, 1, D, dtype, scale=scale))
+    for t in range(n):
+        s = np.sign(scale) * k[:t + 1, 0]
+        want = v[:t + 1][s == s.max()].mean(0)
+        assert np.abs(got[t] - want).max() <= 8 * 2 * half_step(dtype) + 1e-6
+
+
 def test_prompt_attn_values_of_very_different_sizes():
     """by prompt, and by tile of a prompt: f32 rows are scaled by tile"""
     check([200, 100, 150], 4, 2, 64, vkv.F32, v_gain=lambda t: np.where(t < 200, 1e-12, np.where(t < 300, 1e9, 1.0)))

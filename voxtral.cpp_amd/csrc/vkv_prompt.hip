@@ -303,7 +303,7 @@ template <typename T, int D> struct Rows {
     uint4 q[Operand<T>::planes][D / 16], p[Operand<T>::planes][keys / 16];
     floatx16 o[D / 32], s[keys / 32];
     float factor, m, l;
-    int ev_ref;
+    int ev_ref, large;
     int token, t_first, t_last;
     int first_tile, last_tile;      // of those the wave sees
 };
@@ -425,6 +425,7 @@ __device__ __forceinline__ void weights(const PromptArgs &a, int kt, TileInfo in
 #pragma unroll
         for (int t = 0; t < ND; ++t) r.o[t] *= g;
         r.m = m_new;
+        r.large = __any(m_new > -INFINITY && fabsf(m_new) > 0x1p20f);
     }
     float pfac = 1.0f;
     if constexpr (NP == 2) {
@@ -437,13 +438,25 @@ __device__ __forceinline__ void weights(const PromptArgs &a, int kt, TileInfo in
         }
         pfac = ldexpf(1.0f, kPExp + ev - r.ev_ref);
     }
-    const float m_use = r.m > -INFINITY ? -r.m : 0.0f;
+    float by = f, from = r.m > -INFINITY ? -r.m : 0.0f;
+    if (r.large) {
+        // the maximum's own rounding would show in the largest weights: every
+        // score is rounded as it was
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int i = 0; i < KEYS / 2; ++i) {
+            const float x = r.s[i >> 4][i & 15] * f;
+            r.s[i >> 4][i & 15] = x + from;
+        }
+        by = 1.0f;
+        from = 0.0f;
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(r.s[u >> 1][(u & 1) * 8 + i], f, m_use));
+            const float e = __builtin_amdgcn_exp2f(fmaf(r.s[u >> 1][(u & 1) * 8 + i], by, from));
             r.l += e;
             x[i] = NP == 2 ? e * pfac : e;
         }
@@ -555,6 +568,7 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     r.m = -INFINITY;
     r.l = 0.0f;
     r.ev_ref = -1000;
+    r.large = 0;
 
     wait_for_memory();
     meet();
