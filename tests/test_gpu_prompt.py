@@ -84,8 +84,8 @@ def test_prompt_attn_many_prompts():
 
 
 @pytest.mark.parametrize("n", [63, 64, 65])
-def test_prompt_attn_of_prompts_in_order_of_length(n):
-    """up to 64 prompts are taken by length, more in their order"""
+def test_prompt_attn_of_about_64_prompts(n):
+    """the search for a tile's prompt takes one step up to 64 prompts, then two"""
     rng = np.random.default_rng(n)
     lens = list(rng.integers(0, 20, n))
     lens[3], lens[n // 2], lens[-1] = 200, 333, 131

@@ -381,6 +381,11 @@ __global__ __launch_bounds__(THREADS) void k_page_map_small(MapArgs a) {
     }
 }
 
+// The map's own work group does the tokens too where they are so many turns of
+// its threads at the most (32 requests, 64 tokens: 4.0 us, 5.3 with a second
+// launch; 401 of up to 4000: 8.5 and 9.8; 64 of up to 1800, 28 turns: 18.5 and
+// 7.2).
+constexpr int kMapInlineTurns = 4;
 constexpr int kMapOffsets = 4096;    // that k_map_tokens keeps in LDS
 
 // Slots and positions of many tokens, after the map itself, by a search in
@@ -1065,9 +1070,13 @@ template <typename T, int FMT, int D> hipError_t attn_launch(const PagedAttnArgs
     return hipGetLastError();
 }
 
-template <typename T, int FMT, int D> hipError_t append_launch(const AppendPagesArgs &a, hipStream_t st) {
+constexpr int64_t kAppendGroups = 2048;
+
+template <typename T, int FMT, int D> hipError_t append_launch(AppendPagesArgs a, hipStream_t st) {
     const int waves = a.page_size / 16 > 4 ? a.page_size / 16 : 4, units = waves / (a.page_size / 16);
-    const dim3 grid((unsigned)((a.n_tokens + a.looks - 1) / a.looks), (unsigned)((2 * a.n_kv_heads + units - 1) / units));
+    const int64_t heads = (2 * a.n_kv_heads + units - 1) / units;
+    for (a.looks = 1; a.looks < 64 && a.looks < a.page_size && heads * a.n_tokens > kAppendGroups * a.looks;) a.looks *= 2;
+    const dim3 grid((unsigned)((a.n_tokens + a.looks - 1) / a.looks), (unsigned)heads);
     k_pages_append<T, FMT, D><<<grid, 64 * waves, 0, st>>>(a);
     return hipGetLastError();
 }
@@ -1090,7 +1099,8 @@ template <typename F> hipError_t by_types(int dtype, int code, int head_dim, F f
 }  // namespace
 
 hipError_t launch_page_map(const MapArgs &a, hipStream_t st) {
-    const bool inl = a.max_tokens <= kMapInlineTokens;
+    const int threads = a.n_req <= 64 ? 64 : a.n_req <= 256 ? 256 : 1024;
+    const bool inl = a.max_tokens <= kMapInlineTurns * threads;
     if (a.n_req <= 64)
         inl ? k_page_map_small<64, false><<<1, 64, 0, st>>>(a) : k_page_map_small<64, true><<<1, 64, 0, st>>>(a);
     else if (a.n_req <= 256)

@@ -18,7 +18,6 @@
 #include <cfloat>
 
 #include "vkv_serve.h"
-#include "vkv_wave.h"
 
 namespace vkv {
 namespace {
@@ -135,36 +134,6 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs &a, int64_t slot, i
     p.start = offset_of(a, p.seq);
     p.n = max(offset_of(a, p.seq + 1) - p.start, 0);
     p.local = (int)(slot - ((int64_t)p.start * mul / per + p.seq));
-    return true;
-}
-
-// Up to 64 prompts, a lane each: their query tiles by falling number of keys,
-// place by place over all prompts, so that a long prompt's last tiles do not
-// begin when the others have ended (13 prompts of up to 1021 tokens, f32:
-// MEASURE).
-__device__ __forceinline__ bool find_longest(const PromptArgs &a, int at, int mul, int per, Prompt &p) {
-    const int lane = threadIdx.x & 63;
-    const int start = offset_of(a, min(lane, a.n_seq));
-    const int n = lane < a.n_seq ? max(offset_of(a, min(lane, a.n_seq - 1) + 1) - start, 0) : 0;
-    const int tiles = (int)(((int64_t)n * mul + per - 1) / per);
-    // tiles at place `low` or behind it: more than `at`, at place `high`: not
-    // (all of them are fewer than 2^24)
-    auto from = [&](int place) { return __builtin_amdgcn_readfirstlane((int)wave_sum((float)max(tiles - place, 0))); };
-    if (at >= from(0)) return false;
-    int low = 0, high = __builtin_amdgcn_readfirstlane((int)wave_max((float)tiles));
-    while (high - low > 1) {
-        const int mid = (low + high) / 2;
-        if (from(mid) > at) low = mid; else high = mid;
-    }
-    const int nth = at - from(low + 1);
-    const unsigned long long there = __ballot(tiles > low);
-    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(there >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)there, 0));
-    const unsigned long long it = __ballot(tiles > low && before == nth);
-    if (it == 0) return false;      // (offsets that are none, with more tiles than can be counted)
-    p.seq = __ffsll(it) - 1;
-    p.start = __builtin_amdgcn_readlane(start, p.seq);
-    p.n = __builtin_amdgcn_readlane(n, p.seq);
-    p.local = low;
     return true;
 }
 
@@ -491,10 +460,9 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     const int group = a.n_q_heads / a.n_kv_heads;
     const int head = blockIdx.x % a.n_kv_heads;
     // the later tiles of a prompt have the most keys: they go first
-    const int at = blockIdx.x / a.n_kv_heads;
+    const int64_t slot = a.n_slots - 1 - blockIdx.x / a.n_kv_heads;
     Prompt p;
-    if (!(a.n_seq <= 64 ? find_longest(a, at, group, kPromptRows, p) : find_prompt(a, a.n_slots - 1 - at, group, kPromptRows, p)))
-        return;
+    if (!find_prompt(a, slot, group, kPromptRows, p)) return;
     // a call's rows are fewer than 2^31
     const unsigned rows = (unsigned)p.n * (unsigned)group;
     const unsigned row0 = (unsigned)p.local * kPromptRows;

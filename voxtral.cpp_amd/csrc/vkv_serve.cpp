@@ -199,7 +199,6 @@ vkv_status vkv_pages_append(const vkv_pages *pages, int32_t layer, const int32_t
     a.n_slots = pages->n_pages * pages->page_size;
     a.page_size = pages->page_size;
     a.n_kv_heads = pages->n_kv_heads;
-    a.looks = n_tokens <= kAppendAlone ? 1 : std::min(pages->page_size, 64);
     StreamDevice on(as_stream(hip_stream));
     const hipError_t e = launch_pages_append(dtype, pages->dtype, pages->head_dim, a, as_stream(hip_stream));
     if (e != hipSuccess) return host_hip_fail(e, "pages append launch");

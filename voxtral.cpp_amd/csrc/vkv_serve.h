@@ -11,9 +11,6 @@
 
 namespace vkv {
 
-// Up to so many new tokens, vkv_page_map is one launch.
-constexpr int kMapInlineTokens = 4096;
-
 struct MapArgs {
     const int32_t *len_old, *len_new;
     int32_t n_req, page_size, n_pages;
@@ -37,9 +34,6 @@ struct AppendPagesArgs {
     int32_t n_tokens, n_slots, page_size, n_kv_heads;
     int32_t looks;         // tokens that a work group looks at for first ones of their page (<= 64)
 };
-// Up to so many tokens, an append has a work group (per few heads) for each.
-constexpr int kAppendAlone = 512;
-
 hipError_t launch_pages_append(int dtype, int code, int head_dim, const AppendPagesArgs &a, hipStream_t st);
 
 // Keys per work group of the paged attention: a multiple of the 128 keys its
