@@ -882,8 +882,8 @@ vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *
  * does not attend to have no effect on it, NaN and infinities among them (in
  * F32 but for the bits below).
  * F32 rows are multiplied as pairs of f16: 22 bits of a value that is within
- * 2^-16 of the largest of its q row and head or, in k and v, of its kv head's
- * 32 or 64 neighbouring keys; steps of 2^-38 of that largest below.  F16 and
+ * 2^-15 of the largest of its q row and head or, in k and v, of its kv head's
+ * 32 or 64 neighbouring keys; steps of 2^-37 of that largest below.  F16 and
  * BF16 rows are multiplied as they are, with the softmax weights rounded to
  * that type.  Sums are 32-bit.
  * The workspace is 256-byte aligned; its contents do not matter. */

@@ -148,15 +148,22 @@ template <typename T> __device__ __noinline__ void pick(const T *x, int64_t from
     }
 }
 
-// A work group takes `turns` pieces of BLOCKS 16-byte blocks per thread,
-// counted from the 16-byte boundary at or below the row's first element; the
-// next piece is on its way while one is worked on.
+// log p_t = x_t - m - log s, entropy = log s - t / s with s = sum exp(x - m), t =
+// sum (x - m) exp(x - m).  A work group takes `turns` pieces of BLOCKS 16-byte
+// blocks per thread, counted from the 16-byte boundary at or below the row's
+// first element; the next piece is on its way while one is worked on.
 //
 // A value that n of the 256 threads' maxima reach is reached by n elements at
 // least, so nothing below it is among the n largest.  Found once, in the first
-// piece, by one wave while the others sum, it is the limit for all.  The blocks with elements that are not below
-// it, a few more than n per piece as a rule, are set aside whole, one test for
-// a block; at the end their elements go to a list that is ranked by counting.
+// piece, by one wave while the others sum, it is the limit for all.  The blocks
+// with elements that are not below it, a few more than n per piece as a rule,
+// are set aside whole, one test for a block; at the end their elements go to a
+// list that is ranked by counting.
+//
+// Bound by the vector units beside the loads, about 8 instructions and one
+// exponential for an element: 251 rows of 131072 logits in bf16 with 20
+// alternatives 19 us, 3.5 TB/s (12 us without alternatives).  One f32 row 5.2
+// us: a launch, a load, a search and a ranking.
 template <typename T, int BLOCKS>
 __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
     constexpr int EB = 16 / (int)sizeof(T);     // elements of a block
@@ -324,7 +331,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
 // wave's fit its piece
 constexpr int kJoinPer = 3;
 
-// A work group per row.
+// A work group per row.  Latency: statistics and lists, the token's logit, a
+// search and a ranking (one row 4.4 us, 251 rows with 20 alternatives 5.0 us).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
     __shared__ List list;

@@ -90,10 +90,11 @@ __device__ __forceinline__ void map_token(const MapArgs &a, int t, int r, int po
 }
 
 // Any number of requests.  One work group: the free stack is one list, and a
-// step's lengths are a few KB.  Pass 1 sums what the step moves and checks it; nothing is written
-// before the whole step is known to fit.  Pass 2 pushes the returned pages,
-// pass 3 pops the taken ones; both spread the moved pages (not the requests)
-// over the threads, by a search in the scanned counts.
+// step's lengths are a few KB.  Pass 1 sums what the step moves and checks it;
+// nothing is written before the whole step is known to fit.  Pass 2 pushes the
+// returned pages, pass 3 pops the taken ones; both spread the moved pages (not
+// the requests) over the threads, by a search in the scanned counts.  Bound by
+// the latency of its passes' loads and barriers (1000 requests 13.1 us).
 // NOTOKENS: the tokens' slots are left to k_map_tokens.
 template <bool NOTOKENS>
 __global__ __launch_bounds__(kMapThreads) void k_page_map(MapArgs a) {
@@ -246,8 +247,10 @@ __device__ __forceinline__ int wave_scan(int x) {
 // The same as k_page_map for as many requests as threads: a request is a
 // thread's from the first load to the last store, the three sums are scanned
 // together, and a step of single tokens (the usual one) needs no search and
-// two trips to memory, lengths and then pages.  The time is latency: 32
-// requests take one wave, whose barriers cost nothing.
+// two trips to memory, lengths and then pages.  The time is latency, so the
+// fewest threads are the fastest: 32 requests 4.0 us with 64 threads, 5.9 with
+// 1024, 11.1 by k_page_map; 200 requests 4.7 us with 256, 5.9 with 1024; 1000
+// requests 6.6 us, 13.1 by k_page_map.
 template <int THREADS, bool NOTOKENS>
 __global__ __launch_bounds__(THREADS) void k_page_map_small(MapArgs a) {
     constexpr int WAVES = THREADS / 64;
@@ -389,7 +392,8 @@ constexpr int kMapInlineTurns = 4;
 constexpr int kMapOffsets = 4096;    // that k_map_tokens keeps in LDS
 
 // Slots and positions of many tokens, after the map itself, by a search in
-// the offsets.
+// the offsets, which stay in LDS where they fit (65536 places for 401 requests
+// 3.6 us: latency).
 __global__ __launch_bounds__(256) void k_map_tokens(MapArgs a) {
     __shared__ int cu[kMapOffsets];
     const int n = a.n_req;
@@ -503,16 +507,21 @@ template <typename T, int N> struct Raw {
     __device__ float operator[](int i) const { return to_f32(((const T *)w)[i]); }
 };
 
-// The run of tokens that a page's rows come in: the work group of the run's
-// first token does it all; `looks` tokens are a work group's to look at for
-// first ones (one where the tokens are few, so that each has a work group of
-// its own; a page's worth where most tokens are in the middle of a run).
+// code = round(x 2^-e), e the least exponent that holds the page's largest
+// magnitude.  The run of tokens that a page's rows come in: the work group of
+// the run's first token does it all; `looks` tokens are a work group's to look
+// at for first ones.
 //
 // A wave owns one 16-token block of one (page, K or V, head), so a block's
 // rows are read once and stay in registers between the search for the largest
 // magnitude and the rounding; S / 16 waves share a page and meet in LDS.  Lane
 // (g, c) has rows 4 g + j and dims [c D/16, (c + 1) D/16): four tokens of a
 // dim are a word of V's stored order.
+//
+// Few tokens are bound by latency: slots, rows, and the page's waves' meeting
+// (32 of 8 x 128 f32 values 4.8 us, 2.5 of them an empty launch's).  4099
+// tokens of prompts, bf16 to int8 pages of 64: 14 us for 25 MB, 1.8 TB/s: the
+// search for the runs ends after 5.0 us, the rows are there after 9.9.
 template <typename T, int FMT, int D>
 __global__ __launch_bounds__(1024) void k_pages_append(AppendPagesArgs a) {
     constexpr int N = D / 16;
@@ -887,6 +896,23 @@ __device__ __forceinline__ void attn_steps(uint8_t *k0, uint8_t *k1, uint8_t *v0
     }
 }
 
+// out = sum_j 2^(s_j - m) V_j / sum_j 2^(s_j - m), s_j = scale log2 e q . K_j,
+// in one pass over the keys with a running maximum m.  A work group takes a
+// chunk of a row's keys for up to 8 query heads of a kv head, its waves 32 keys
+// at a time in turn; DIRECT: one chunk is the row.  Both products are
+// v_mfma_f32_16x16x32_f16: codes are exact in f16; q and the weights take two
+// columns each, the value in f16 and what that leaves (times 2^11), so that the
+// 16 columns are 8 heads and nothing is multiplied twice.  A V scale is a power
+// of two and goes into the weights.
+//
+// Bound by the codes' way from HBM (32 flop for a byte: the matrix cores are
+// busy for less than a tenth of the time).  Codes go into LDS without registers, two steps
+// ahead (32 KiB per wave in flight for D 128), past the caches' order, by whole
+// lines.  64 ragged requests of up to 8192 tokens (8 kv heads of 128, 575 MB)
+// 116 us, 5.0 TB/s; 64 x 8192 tokens 5.1 to 5.9 TB/s; 131 rows of 32 heads of
+// 64 in a window of 750 68 us, 4.6 TB/s; one row of 8192 tokens (17 MB) 8.7 us,
+// a launch, the table, and two steps' latency.  A copy of 1 GiB runs at 5.06
+// TB/s, reads alone at 5.8 to 6.7.
 template <typename T, int FMT, int D, int WAVES, bool DIRECT>
 __global__ __launch_bounds__(64 * WAVES) void k_paged_attn(PagedAttnArgs a) {
     constexpr int NM = D / 32, NT = D / 16;
@@ -1002,7 +1028,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_paged_attn(PagedAttnArgs a) {
 }
 
 // Joins the chunks of a (row, query head): a wave's lanes read the chunks'
-// maxima and sums, 64 at a time, then all their parts of the output at once.
+// maxima and sums, 64 at a time, then 16 of their parts of the output at once.
+// Latency: 32 chunks of 32 heads 4.0 us, as 2 or 3 trips to memory take.
 template <typename T, int D>
 __global__ __launch_bounds__(64) void k_paged_merge(PagedAttnArgs a) {
     constexpr int V = D / 64;       // dims per lane
@@ -1070,6 +1097,12 @@ template <typename T, int FMT, int D> hipError_t attn_launch(const PagedAttnArgs
     return hipGetLastError();
 }
 
+// A work group looks at as few tokens as leave this many work groups: each of
+// its first tokens is a chain of loads (1000 requests of one token each 15.5
+// us, 36 where a work group looks at 16; 512 tokens of prompts in pages of 64
+// 10.0 us, 15.3 where it looks at one, 10.5 with half the work groups), and a
+// page's worth of tokens at the most (4099 tokens as above 13.9 us, 15.0 where
+// it looks at 32, 49 where it looks at one).
 constexpr int64_t kAppendGroups = 2048;
 
 template <typename T, int FMT, int D> hipError_t append_launch(AppendPagesArgs a, hipStream_t st) {
