@@ -296,6 +296,30 @@ def test_logprobs_of_many_rows_of_every_kind(dtype):
         assert np.isnan(got[0][r]) and np.isnan(got[1][r]) and np.isnan(got[3][r]).all() and got[2][r, 0] == first
 
 
+@pytest.mark.parametrize("dtype", [vkv.F32, vkv.F16])
+@pytest.mark.parametrize("vocab,rows", [(7, 3), (5000, 5), (20001, 300)])
+def test_logprobs_of_rows_that_are_sure(vocab, rows, dtype):
+    """a probability next to 1: its logarithm and the entropy to f32's relative precision.  The other terms' sum has
+    terms off by |x - m| 2^-24 (their arguments, below 40 here) and 2 2^-24, and is one in trees as above; the logarithm
+    and the division add 3 2^-24; the entropy's terms are these and their products with |x - m|, all of one sign"""
+    rng = np.random.default_rng(15)
+    x = rng.uniform(-3, 3, (rows, vocab))
+    token = rng.integers(0, vocab, rows)
+    x[np.arange(rows), token] = np.arange(rows) % 20 + 12
+    dev_x = rows_on_device(x, dtype)
+    got = logprobs(dev_x, token, 1, dtype)
+    x = as64(dev_x)
+    d = x - x[np.arange(rows), token][:, None]
+    e = np.exp(d)
+    e[np.arange(rows), token] = 0
+    rest = e.sum(1)
+    lp = -np.log1p(rest)
+    ent = np.log1p(rest) - (e * d).sum(1) / (1 + rest)
+    rel = (40 + 2 + 32 + np.log2(vocab) + 3) * 2.0 ** -24
+    assert (np.abs(got[0] - lp) <= rel * np.abs(lp)).all() and np.array_equal(got[0], got[3][:, 0])
+    assert (np.abs(got[1] - ent) <= 2 * rel * ent).all()
+
+
 @pytest.mark.parametrize("vocab,rows", [(5000, 5), (20001, 300)])
 def test_logprobs_of_large_logits(vocab, rows):
     """spread over, or all near, magnitudes at which a unit is many, few and none of f32's steps"""

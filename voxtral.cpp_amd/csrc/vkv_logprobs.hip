@@ -3,7 +3,7 @@
 //
 // k_logprobs_part: a work group takes a chunk of a row into registers; each of
 // its waves sums exp(x - max) and (x - max) exp(x - max) against its own
-// maximum, and the work group picks its n_top largest elements.
+// maximum (whose own terms it counts), and the work group picks its n_top largest elements.
 // k_logprobs_join: a work group per row joins the waves' sums and the chunks'
 // lists.
 #include <hip/hip_runtime.h>
@@ -162,8 +162,9 @@ template <typename T> __device__ __noinline__ void pick(const T *x, int64_t from
 //
 // Bound by the vector units beside the loads, about 8 instructions and one
 // exponential for an element: 251 rows of 131072 logits in bf16 with 20
-// alternatives 19 us, 3.5 TB/s (12 us without alternatives).  One f32 row 5.2
-// us: a launch, a load, a search and a ranking.
+// alternatives 21 us, 3.1 TB/s (12 us without alternatives), 2 of them for the
+// maximum's terms kept apart.  One f32 row 5.3 us: a launch, a load, a search
+// and a ranking.
 template <typename T, int BLOCKS>
 __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
     constexpr int EB = 16 / (int)sizeof(T);     // elements of a block
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
     };
     uint4 next[BLOCKS];
     load(chunk0, next);
-    float m = -INFINITY, s = 0.0f, t = 0.0f, limit = -INFINITY, largest = -INFINITY;
+    float m = -INFINITY, s = 0.0f, t = 0.0f, n = 0.0f, limit = -INFINITY, largest = -INFINITY;
     int kept = 0, set_aside = 0;
     for (int piece = chunk0; piece < end; piece += PIECE) {
         float v[PER];
@@ -228,37 +229,53 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
         const float m_new = fmaxf(m, wave_max(mine));
         const float ref = m_new > -INFINITY ? m_new : 0.0f;
         // the sums so far move to the new maximum (without a term: none)
-        if (m_new > m && s != 0.0f) {
+        if (m_new > m && s + n != 0.0f) {
             const float d = (m - ref) * kLog2e, f = __builtin_amdgcn_exp2f(d);
-            t = f != 0.0f ? f * fmaf(d, s, t) : 0.0f;
-            s *= f;
+            t = f != 0.0f ? f * fmaf(d, s + n, t) : 0.0f;
+            s = (s + n) * f;
+            n = 0.0f;
         }
         m = m_new;
         // exp(x - ref) = 2^d, d = x log2 e - c in one rounding; what c's own
         // lacks is the same for every term and comes off the sums
-        const float c = ref * kLog2e;
-        float lack = fmaf(ref, kLog2e, -c), s1 = 0.0f, t1 = 0.0f;
+        const float c = ref * kLog2e, top = fabsf(m) <= FLT_MAX ? m : __builtin_nanf("");
+        float lack = fmaf(ref, kLog2e, -c), s1 = 0.0f, t1 = 0.0f, n1 = 0.0f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const float d = fmaf(v[i], kLog2e, -c), e = __builtin_amdgcn_exp2f(d);
-            s1 += e;
-            t1 = fmaf(e, d, t1);
+        for (int b = 0; b < BLOCKS; ++b) {
+            if (__any(of_block[b] == top)) {
+#pragma unroll
+                for (int i = 0; i < EB; ++i) {
+                    const float x = v[b * EB + i], d = fmaf(x, kLog2e, -c), e = __builtin_amdgcn_exp2f(d);
+                    s1 += x == top ? 0.0f : e;
+                    t1 = fmaf(x == top ? 0.0f : e, d, t1);
+                    n1 += x == top ? 1.0f : 0.0f;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < EB; ++i) {
+                    const float d = fmaf(v[b * EB + i], kLog2e, -c), e = __builtin_amdgcn_exp2f(d);
+                    s1 += e;
+                    t1 = fmaf(e, d, t1);
+                }
+            }
         }
         if (__any(!(fabsf(t1) <= FLT_MAX && fabsf(lack) <= 1.0f))) {
             // a logit of -inf (0 times the logarithm of 0 is 0), or one so
             // large that c lacks whole powers of two: d from the difference
-            lack = s1 = t1 = 0.0f;
+            lack = s1 = t1 = n1 = 0.0f;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                const float d = (v[i] - ref) * kLog2e, e = __builtin_amdgcn_exp2f(d);
+                const float d = (v[i] - ref) * kLog2e, e = v[i] == top ? 0.0f : __builtin_amdgcn_exp2f(d);
                 s1 += e;
                 t1 = fmaf(e, fmaxf(d, -200.0f), t1);
+                n1 += v[i] == top ? 1.0f : 0.0f;
             }
         }
         t1 = fmaf(-lack, s1, t1);
         lack = __builtin_amdgcn_exp2f(-lack);
         s = fmaf(s1, lack, s);
         t = fmaf(t1, lack, t);          // in log2 units
+        n += n1;
         if (a.n_top == 0) continue;
         if (looks) {
             __syncthreads();
@@ -294,6 +311,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
     }
     s = wave_sum(s);
     t = wave_sum(t);
+    n = wave_sum(n);
     if (limit > -INFINITY && a.turns * a.n_top > kFewKeys) {
         // the limit again, from all pieces: a list of few is ranked sooner
         __syncthreads();
@@ -314,7 +332,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
         }
     }
     if ((tid & 63) == 0) {
-        *((float4 *)a.stats + ((int64_t)row * a.n_chunks + chunk) * kWaves + (tid >> 6)) = float4{m, s, t * kLn2, 0.0f};
+        *((float4 *)a.stats + ((int64_t)row * a.n_chunks + chunk) * kWaves + (tid >> 6)) = float4{m, s, t * kLn2, n};
         list.count[tid >> 6] = min(kept, kPiece);
         wave_odd[tid >> 6] = s != s || kept > kPiece || set_aside > kHot;   // NaN or +inf, or a full list
     }
@@ -331,8 +349,27 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
 // wave's fit its piece
 constexpr int kJoinPer = 3;
 
+// A wave's, or several waves', elements: the maximum m, how many there are of
+// it, and of the others the sums of exp(x - m) and (x - m) exp(x - m).  The
+// maximum's own terms are kept apart because in a row that is sure of its
+// token they are all but the whole sum: log(n + s) = log n + log1p(s / n) then
+// has the others' part in full.
+struct Sums {
+    float m, s, t, n;
+    // to the maximum `to`, which is not below m; what has no term, or weighs
+    // nothing, adds nothing
+    __device__ __forceinline__ void bring(float to) {
+        if (m == to) return;
+        const float d = m - to, f = expf(d), all = s + n;
+        t = all != 0.0f && f != 0.0f ? f * (t + d * all) : 0.0f;
+        s = all != 0.0f ? f * all : 0.0f;
+        n = 0.0f;
+        m = to;
+    }
+};
+
 // A work group per row.  Latency: statistics and lists, the token's logit, a
-// search and a ranking (one row 4.4 us, 251 rows with 20 alternatives 5.0 us).
+// search and a ranking (one row 4.7 us, 251 rows with 20 alternatives 5.2 us).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
     __shared__ List list;
@@ -354,32 +391,27 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
     const int token = a.tokens ? a.tokens[row] : -1;
     const bool is_token = token >= 0 && token < a.n_vocab;
     const float at_token = is_token ? (float)((const T *)a.logits)[row * a.row_stride + token] : 0.0f;
-    float m = -INFINITY, s = 0.0f, t = 0.0f;
+    Sums sums{-INFINITY, 0.0f, 0.0f, 0.0f};
     for (int i = tid; i < n_stats; i += kThreads) {
-        const float4 x = st[i];
-        const float to = fmaxf(m, x.x), ref = to > -INFINITY ? to : 0.0f;
-        const float dm = (m > -INFINITY ? m : 0.0f) - ref, dx = (x.x > -INFINITY ? x.x : 0.0f) - ref;
-        const float fm = expf(dm), fx = expf(dx);
-        // both sums move to the larger maximum; what has no term, or weighs nothing, adds nothing
-        t = (s != 0.0f && fm != 0.0f ? fm * (t + dm * s) : 0.0f) + (x.y != 0.0f && fx != 0.0f ? fx * (x.z + dx * x.y) : 0.0f);
-        s = (s != 0.0f ? fm * s : 0.0f) + (x.y != 0.0f ? fx * x.y : 0.0f);
-        m = to;
+        const float4 y = st[i];
+        Sums more{y.x, y.y, y.z, y.w};
+        const float to = fmaxf(sums.m, more.m);
+        sums.bring(to);
+        more.bring(to);
+        sums.s += more.s;
+        sums.t += more.t;
+        sums.n += more.n;
     }
-    const float wm = wave_max(m);
+    const float wm = wave_max(sums.m);
     if ((tid & 63) == 0) red[tid >> 6][0] = wm;
     __syncthreads();
-    const float top_m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
-    const float ref = top_m > -INFINITY ? top_m : 0.0f;
-    {
-        const float d = (m > -INFINITY ? m : 0.0f) - ref, f = expf(d);
-        t = s != 0.0f && f != 0.0f ? f * (t + d * s) : 0.0f;
-        s = s != 0.0f ? f * s : 0.0f;
-    }
-    s = wave_sum(s);
-    t = wave_sum(t);
+    const float ref = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+    sums.bring(ref);
+    const float ws = wave_sum(sums.s), wt = wave_sum(sums.t), wn = wave_sum(sums.n);
     if ((tid & 63) == 0) {
-        red[tid >> 6][1] = s;
-        red[tid >> 6][2] = t;
+        red[tid >> 6][1] = ws;
+        red[tid >> 6][2] = wt;
+        red[tid >> 6][3] = wn;
     }
 
     // the n largest keys: as in a chunk, a turn's worth of keys at a time,
@@ -413,11 +445,12 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
         rank(list, a.n_top, top);
     }
     __syncthreads();
-    s = red[0][1] + red[1][1] + red[2][1] + red[3][1];
-    t = red[0][2] + red[1][2] + red[2][2] + red[3][2];
+    const float s = red[0][1] + red[1][1] + red[2][1] + red[3][1];
+    const float t = red[0][2] + red[1][2] + red[2][2] + red[3][2];
+    const float n = red[0][3] + red[1][3] + red[2][3] + red[3][3];
     // a row of -inf alone: no sum
-    const bool none = s == 0.0f;
-    const float log_s = none ? 0.0f : logf(s);
+    const bool none = n == 0.0f && s == 0.0f;
+    const float log_s = none ? 0.0f : logf(n) + log1pf(s / n);
     auto logprob = [&](float x) { return none ? -INFINITY : (x - ref) - log_s; };
     if (tid < a.n_top) {
         const u64 key = top[tid];
@@ -425,7 +458,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
         a.top_logprobs[(int64_t)row * a.n_top + tid] = logprob(value_of((unsigned)(key >> 32)));
     }
     if (tid == kThreads - 1) {
-        if (a.entropy) a.entropy[row] = none ? 0.0f : log_s - t / s;
+        if (a.entropy) a.entropy[row] = none ? 0.0f : log_s - t / (n + s);
         if (a.tokens) a.logprob[row] = is_token ? logprob(at_token) : token == -1 ? 0.0f : __builtin_nanf("");
     }
 }
