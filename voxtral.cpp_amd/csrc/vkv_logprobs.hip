@@ -102,21 +102,21 @@ struct Hot {
 // its keys are distinct.  A barrier is between the list's writing and this.
 __device__ __forceinline__ void rank(const List &list, int n, u64 *out) {
     const int4 c = *(const int4 *)list.count;
-    const int to1 = c.x, to2 = to1 + c.y, to3 = to2 + c.z, total = to3 + c.w, most = max(max(c.x, c.y), max(c.z, c.w));
+    const int to1 = c.x, to2 = to1 + c.y, to3 = to2 + c.z, total = to3 + c.w;
     for (int i = threadIdx.x; i < total; i += kThreads) {
         const int w = (i >= to1) + (i >= to2) + (i >= to3);
         const u64 k = list.key[w][i - (w == 0 ? 0 : w == 1 ? to1 : w == 2 ? to2 : to3)];
         int above = 0;
-        for (int j = 0; j < most; j += 4) {
-            u64 x[kWaves][4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+        for (int v = 0; v < kWaves; ++v) {
+            const int of_v = v == 0 ? c.x : v == 1 ? c.y : v == 2 ? c.z : c.w;
+            for (int j = 0; j < of_v; j += 4) {
+                u64 x[4];
 #pragma unroll
-                for (int v = 0; v < kWaves; ++v) x[v][q] = list.key[v][j + q];
+                for (int q = 0; q < 4; ++q) x[q] = list.key[v][j + q];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                above += (j + q < c.x && x[0][q] > k) + (j + q < c.y && x[1][q] > k) + (j + q < c.z && x[2][q] > k) +
-                         (j + q < c.w && x[3][q] > k);
+                for (int q = 0; q < 4; ++q) above += j + q < of_v && x[q] > k;
+            }
         }
         if (above < n) out[above] = k;
     }
@@ -299,14 +299,12 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
             }
         } else {
             // fewer than n above -inf: they, and the chunk's first n for those of -inf that rank
-#pragma unroll 1
-            for (int b = 0; b < BLOCKS; ++b)
-                for (int i = 0; i < EB; ++i) {
-                    const int e = piece + (b * kThreads + tid) * EB + i;
-                    const float y = e >= 0 && e < vocab ? (float)x[e] : -INFINITY;
-                    put(list, kept, e >= 0 && e < vocab && (y > -INFINITY || e - begin < a.n_top),
-                        [&] { return key_of(y, (unsigned)e); });
-                }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int e = piece + ((i / EB) * kThreads + tid) * EB + i % EB;
+                put(list, kept, e >= 0 && e < vocab && (v[i] > -INFINITY || e - begin < a.n_top),
+                    [&] { return key_of(v[i], (unsigned)e); });
+            }
         }
     }
     s = wave_sum(s);
