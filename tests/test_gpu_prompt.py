@@ -197,6 +197,50 @@ def test_prompt_attn_offsets_outside_the_rows_are_held_to_them():
     assert torch.equal(got[90:], want[90:]) and (got[:90] == 7.0).all()
 
 
+@pytest.fixture
+def many_groups(monkeypatch):
+    """200 empty prompts behind the others: the form for many work groups takes what the other form took above"""
+    real = call
+
+    def padded(q, k, v, cu, *rest, **kw):
+        return real(q, k, v, list(cu) + [cu[-1]] * 200, *rest, **kw)
+    monkeypatch.setitem(globals(), "call", padded)
+
+
+@pytest.mark.parametrize("dtype", [vkv.F32, vkv.F16, vkv.BF16])
+@pytest.mark.parametrize("H,Hk,D", [(8, 2, 128), (4, 4, 64), (9, 3, 64), (16, 1, 128)])
+def test_prompt_attn_many_groups_ragged(H, Hk, D, dtype, many_groups):
+    check([1, 0, 2, 63, 64, 65, 0, 0, 127, 128, 129, 31, 38, 300], H, Hk, D, dtype)
+
+
+@pytest.mark.parametrize("window", [1, 31, 64, 65, 100, 500])
+@pytest.mark.parametrize("dtype,D", [(vkv.F32, 128), (vkv.F32, 64), (vkv.F16, 64)])
+def test_prompt_attn_many_groups_window(window, dtype, D, many_groups):
+    check([150, 1, 333, 64], 4, 2, D, dtype, window)
+
+
+@pytest.mark.parametrize("dtype", [vkv.F32, vkv.F16, vkv.BF16])
+def test_prompt_attn_many_groups_of_every_kind(dtype, many_groups):
+    for window in (0, 30):
+        test_prompt_attn_keys_out_of_sight_do_nothing(dtype, window)
+    for scale in (1e6, -1e8, 1e20):
+        test_prompt_attn_of_scores_beyond_their_own_steps(dtype, scale)
+    if dtype == vkv.F32:
+        for gain, scale in ((300.0, None), (1e-30, None), (1.0, -0.1), (1.0, 0.0), (1e30, 1e-31)):
+            test_prompt_attn_of_scores_far_apart(gain, scale)
+        test_prompt_attn_values_of_very_different_sizes()
+        test_prompt_attn_offsets_outside_the_rows_are_held_to_them()
+        test_prompt_attn_of_more_than_64_tiles(0)
+    test_prompt_attn_rows_of_one_wide_array()
+
+
+@pytest.mark.parametrize("dtype", [vkv.F32, vkv.F16, vkv.BF16])
+@pytest.mark.parametrize("D,n", [(64, 4300), (128, 2200)])
+def test_prompt_attn_of_few_rows_and_many_tiles(dtype, D, n):
+    """more than 64 tiles of keys, four waves on them; one query head, so that the rows are few"""
+    check([n], 1, 1, D, dtype, window=n - 100)
+
+
 # ---- log probabilities ----
 def logprobs(x, tokens, top, dtype, row_stride=0, vocab=None, rows=None):
     n, v = x.shape[0] if rows is None else rows, x.shape[1] if vocab is None else vocab

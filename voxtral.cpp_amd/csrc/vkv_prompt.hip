@@ -306,6 +306,25 @@ template <typename T, int D> __device__ __forceinline__ void scores(Rows<T, D> &
         }
 }
 
+// V's values that are not finite, left out of the product: the rows that see
+// their key take them as they are.
+template <typename T, int D>
+__device__ __forceinline__ void strange_values(const PromptArgs &a, const Prompt &p, int head, int kt, Rows<T, D> &r) {
+    constexpr int KEYS = Rows<T, D>::keys;
+#pragma unroll 1
+    for (int key = kt * KEYS; key < (kt + 1) * KEYS && key < p.n; ++key) {
+        const bool in = key <= r.token && (a.window <= 0 || key > r.token - a.window);
+        const T *x = (const T *)a.v + (p.start + key) * a.v_stride + head * D + 4 * (int)((threadIdx.x & 63) >> 5);
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float y = (float)x[32 * t + 8 * (i >> 2) + (i & 3)];
+                if (in && !(fabsf(y) <= FLT_MAX)) r.o[t][i] += y;
+            }
+    }
+}
+
 // The matrix cores' half of a tile: O^T += V^T P^T for the tile whose weights
 // are at hand, and the scores of the next.  The next tile's operands are
 // fetched into the other places on the way: the four are restrict, or each
@@ -345,22 +364,7 @@ __device__ __forceinline__ void products(const PromptArgs &a, const Prompt &p, i
         __builtin_amdgcn_sched_group_barrier(0x008, NP == 2 ? 3 : 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, NP, 0);
     }
-    if (odd) {
-        // values that are not finite, left out of the product: the rows that
-        // see their key take them as they are
-#pragma unroll 1
-        for (int key = kt * KEYS; key < (kt + 1) * KEYS && key < p.n; ++key) {
-            const bool in = key <= r.token && (a.window <= 0 || key > r.token - a.window);
-            const T *x = (const T *)a.v + (p.start + key) * a.v_stride + head * D + 4 * (lane >> 5);
-#pragma unroll
-            for (int t = 0; t < ND; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float y = (float)x[32 * t + 8 * (i >> 2) + (i & 3)];
-                    if (in && !(fabsf(y) <= FLT_MAX)) r.o[t][i] += y;
-                }
-        }
-    }
+    if (odd) strange_values(a, p, head, kt, r);
 }
 
 // The vector units' half: the scores of tile kt become weights, and the sums
@@ -440,78 +444,32 @@ __device__ __forceinline__ void weights(const PromptArgs &a, int kt, TileInfo in
     }
 }
 
-// A work group: 4 waves on 128 rows of one (prompt, kv head), a row being
-// (token, query head of the kv head), so the heads that share K and V read one
-// copy of them in LDS.  Wave w owns rows 32 w + [0, 32) as the columns of S^T =
-// K Q^T and O^T = V^T P^T; a lane's scores are the keys it supplies to the
-// second product, so P stays in its registers.
-//
-// The products of a tile and the softmax of a tile take about as long, on
-// units that can work at the same time: the registers and the LDS of a work
-// group leave room for a second one on the CU, and each SIMD's two waves, of
-// two work groups that never wait for each other, fill each other's gaps (13
-// prompts of up to 1021 tokens, f32: 168 us, 180 with one work group of two
-// halves that take turns; 38 tokens 9.5 and 15 us).  Operands of tile kt's turn
-// (its V, the K of tile kt + 1) are in LDS at its start; those of the next come
-// in meanwhile.
-//
-// Bound by the matrix cores at the clock that they leave: 8192 tokens of 32
-// heads of 128 in bf16, 550 Gflop, 508 to 540 us with the card, 1.02 to 1.08
-// Pflop/s, where a product of two 8192 x 8192 matrices runs at 1.14; f32, three
-// products, 1.3 ms, 1.26 Pflop/s of f16 products.  13 prompts as above: 153 us,
-// 0.75 Pflop/s: work groups of 11 tiles on average, whose first loads and
-// last stores no work of their own hides.
+// The wave's 32 rows at wrow: their places, the tiles that they see, and this
+// lane's column of Q (dims 16 m + 8 half + [0, 8)) on its way to x; the row's
+// query head of the kv head is returned.
 template <typename T, int D>
-__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_prompt_attn(PromptArgs a) {
-    typedef typename Operand<T>::elem E;
-    constexpr int NP = Operand<T>::planes;
-    constexpr int NM = D / 16, ND = D / 32, KEYS = Rows<T, D>::keys;
-    constexpr int BYTES = tile_bytes<T, D>(), HALF = BYTES / 2;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BYTES];   // K, K, V, V
-
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int half = lane >> 5;
-    const int group = a.n_q_heads / a.n_kv_heads;
-    const int head = blockIdx.x % a.n_kv_heads;
-    // the later tiles of a prompt have the most keys: they go first
-    const int64_t slot = a.n_slots - 1 - blockIdx.x / a.n_kv_heads;
-    Prompt p;
-    if (!find_prompt(a, slot, group, kPromptRows, p)) return;
-    // a call's rows are fewer than 2^31
-    const unsigned rows = (unsigned)p.n * (unsigned)group;
-    const unsigned row0 = (unsigned)p.local * kPromptRows;
-    if (row0 >= rows) return;
-
-    const unsigned wrow = row0 + 32 * wave;
-    const unsigned row = wrow + (lane & 31), row_in = min(row, rows - 1);
-    Rows<T, D> r;
-    r.token = (int)(row_in / (unsigned)group);
-    const int hq = (int)(row_in - (unsigned)r.token * (unsigned)group);
+__device__ __forceinline__ int take_rows(const PromptArgs &a, const Prompt &p, int head, unsigned wrow, unsigned rows, Rows<T, D> &r,
+                                         float (&x)[D / 16][8]) {
+    constexpr int KEYS = Rows<T, D>::keys;
+    const int lane = threadIdx.x & 63, group = a.n_q_heads / a.n_kv_heads;
+    const unsigned row = min(wrow + (lane & 31), rows - 1);
+    r.token = (int)(row / (unsigned)group);
+    const int hq = (int)(row - (unsigned)r.token * (unsigned)group);
     r.t_first = __builtin_amdgcn_readlane(r.token, 0);
     r.t_last = __builtin_amdgcn_readlane(r.token, 31);
     r.first_tile = a.window > 0 && r.t_first >= a.window ? (r.t_first - a.window + 1) / KEYS : 0;
     r.last_tile = wrow < rows ? r.t_last / KEYS : -2;      // a wave without rows sees no key
-    const int wg_first = (int)(row0 / (unsigned)group);
-    const int wg_last = (int)(min(row0 + kPromptRows, rows) - 1) / group;
-    const int kt0 = a.window > 0 && wg_first >= a.window ? (wg_first - a.window + 1) / KEYS : 0;
-    const int kt1 = wg_last / KEYS;
-    const int64_t tile0 = (int64_t)head * a.n_tiles + p.start / KEYS + p.seq;
-    const uint8_t *data = a.data + tile0 * BYTES;
-    // this lane's column of Q: dims 16 m + 8 half + [0, 8)
-    float x[NM][8];
-    const T *q = (const T *)a.q + (p.start + r.token) * a.q_stride + (head * group + hq) * D + 8 * half;
+    const T *q = (const T *)a.q + (p.start + r.token) * a.q_stride + (head * group + hq) * D + 8 * (lane >> 5);
 #pragma unroll
-    for (int m = 0; m < NM; ++m) load8(q + 16 * m, x[m]);
-    // the words of 64 tiles, a lane each: a load for every tile would have the
-    // waits for it cover the operands that are on their way
-    auto tile_words = [&](int kt) { return a.info[tile0 + min(kt + lane, kt1)]; };
-    int words = tile_words(kt0);
-    // K of the first tile where the turn before the first has it, then the first turn's operands
-    fetch<HALF>(data + (int64_t)kt0 * BYTES, lds + HALF, wave);
-    fetch<HALF>(data + (int64_t)min(kt0 + 1, kt1) * BYTES, lds, wave);
-    fetch<HALF>(data + (int64_t)kt0 * BYTES + HALF, lds + 2 * HALF, wave);
+    for (int m = 0; m < D / 16; ++m) load8(q + 16 * m, x[m]);
+    return hq;
+}
 
+// Q in its form, and nothing summed so far.
+template <typename T, int D>
+__device__ __forceinline__ void start_rows(const PromptArgs &a, float (&x)[D / 16][8], Rows<T, D> &r) {
+    typedef typename Operand<T>::elem E;
+    constexpr int NP = Operand<T>::planes, NM = D / 16, ND = D / 32;
     r.factor = fabsf(a.scale) * kLog2e;
     float by = a.scale < 0.0f ? -1.0f : 1.0f;
     bool fine = true;       // the largest value's exponent is that of finite ones
@@ -552,7 +510,70 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     r.l = 0.0f;
     r.ev_ref = -1000;
     r.large = 0;
+}
 
+// A work group: 4 waves on 128 rows of one (prompt, kv head), a row being
+// (token, query head of the kv head), so the heads that share K and V read one
+// copy of them in LDS.  Wave w owns rows 32 w + [0, 32) as the columns of S^T =
+// K Q^T and O^T = V^T P^T; a lane's scores are the keys it supplies to the
+// second product, so P stays in its registers.
+//
+// The products of a tile and the softmax of a tile take about as long, on
+// units that can work at the same time: the registers and the LDS of a work
+// group leave room for a second one on the CU, and each SIMD's two waves, of
+// two work groups that never wait for each other, fill each other's gaps (13
+// prompts of up to 1021 tokens, f32: 168 us, 180 with one work group of two
+// halves that take turns; 38 tokens 9.5 and 15 us).  Operands of tile kt's turn
+// (its V, the K of tile kt + 1) are in LDS at its start; those of the next come
+// in meanwhile.
+//
+// Bound by the matrix cores at the clock that they leave: 8192 tokens of 32
+// heads of 128 in bf16, 550 Gflop, 508 to 540 us with the card, 1.02 to 1.08
+// Pflop/s, where a product of two 8192 x 8192 matrices runs at 1.14; f32, three
+// products, 1.3 ms, 1.26 Pflop/s of f16 products.  13 prompts as above: 153 us,
+// 0.75 Pflop/s: work groups of 11 tiles on average, whose first loads and
+// last stores no work of their own hides.
+template <typename T, int D>
+__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_prompt_attn(PromptArgs a) {
+    constexpr int NP = Operand<T>::planes;
+    constexpr int NM = D / 16, ND = D / 32, KEYS = Rows<T, D>::keys;
+    constexpr int BYTES = tile_bytes<T, D>(), HALF = BYTES / 2;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BYTES];   // K, K, V, V
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5;
+    const int group = a.n_q_heads / a.n_kv_heads;
+    const int head = blockIdx.x % a.n_kv_heads;
+    // the later tiles of a prompt have the most keys: they go first
+    const int64_t slot = a.n_slots - 1 - blockIdx.x / a.n_kv_heads;
+    Prompt p;
+    if (!find_prompt(a, slot, group, kPromptRows, p)) return;
+    // a call's rows are fewer than 2^31
+    const unsigned rows = (unsigned)p.n * (unsigned)group;
+    const unsigned row0 = (unsigned)p.local * kPromptRows;
+    if (row0 >= rows) return;
+
+    Rows<T, D> r;
+    float x[NM][8];
+    const unsigned wrow = row0 + 32 * wave, row = wrow + (lane & 31);
+    const int hq = take_rows(a, p, head, wrow, rows, r, x);
+    const int wg_first = (int)(row0 / (unsigned)group);
+    const int wg_last = (int)(min(row0 + kPromptRows, rows) - 1) / group;
+    const int kt0 = a.window > 0 && wg_first >= a.window ? (wg_first - a.window + 1) / KEYS : 0;
+    const int kt1 = wg_last / KEYS;
+    const int64_t tile0 = (int64_t)head * a.n_tiles + p.start / KEYS + p.seq;
+    const uint8_t *data = a.data + tile0 * BYTES;
+    // the words of 64 tiles, a lane each: a load for every tile would have the
+    // waits for it cover the operands that are on their way
+    auto tile_words = [&](int kt) { return a.info[tile0 + min(kt + lane, kt1)]; };
+    int words = tile_words(kt0);
+    // K of the first tile where the turn before the first has it, then the first turn's operands
+    fetch<HALF>(data + (int64_t)kt0 * BYTES, lds + HALF, wave);
+    fetch<HALF>(data + (int64_t)min(kt0 + 1, kt1) * BYTES, lds, wave);
+    fetch<HALF>(data + (int64_t)kt0 * BYTES + HALF, lds + 2 * HALF, wave);
+
+    start_rows(a, x, r);
     wait_for_memory();
     meet();
     scores(r, lds + HALF);
@@ -596,9 +617,123 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     }
 }
 
+// The same where there are few rows: a work group's 4 waves share 32 rows and
+// take the key tiles in turn, and their parts meet in LDS.  No two waves read
+// the same operands, so they come straight into registers: V's while the
+// scores are made, the next K while they become weights.  Bound by those
+// loads' latency: f32, 32 heads over 8 of 128, 200 tokens 15.8 us with the
+// launch of k_prompt_pack, 21.0 by k_prompt_attn.
+template <typename T, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void k_prompt_attn_few(PromptArgs a) {
+    typedef typename Operand<T>::elem E;
+    constexpr int NP = Operand<T>::planes, NM = D / 16, ND = D / 32, KEYS = Rows<T, D>::keys, KB = KEYS / 32, U = KEYS / 16;
+    constexpr int BYTES = tile_bytes<T, D>(), HALF = BYTES / 2, PIECES = HALF / 1024, PLANE = PIECES / NP;
+    constexpr int OWN = 2 * ND;             // of half of O's 16 ND values per lane, a wave's to join
+    __shared__ float parts[4][4 * OWN][64];
+    __shared__ float lds_m[4][64], lds_l[4][64];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int group = a.n_q_heads / a.n_kv_heads;
+    const int head = blockIdx.x % a.n_kv_heads;
+    Prompt p;
+    if (!find_prompt(a, a.n_slots - 1 - blockIdx.x / a.n_kv_heads, group, kPromptRowsFew, p)) return;
+    const unsigned rows = (unsigned)p.n * (unsigned)group;
+    const unsigned row0 = (unsigned)p.local * kPromptRowsFew, row = row0 + (lane & 31);
+    if (row0 >= rows) return;
+    Rows<T, D> r;
+    float x[NM][8];
+    const int hq = take_rows(a, p, head, row0, rows, r, x);
+    const int kt0 = r.first_tile, kt1 = r.last_tile;
+    const int64_t tile0 = (int64_t)head * a.n_tiles + p.start / KEYS + p.seq;
+    const uint8_t *data = a.data + tile0 * BYTES + lane * 16;
+    int words_at = kt0, words = a.info[tile0 + min(kt0 + lane, kt1)];
+    uint4 k[PIECES], v[PIECES];
+    auto load = [&](uint4 (&to)[PIECES], const uint8_t *from) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) to[i] = *(const uint4 *)(from + i * 1024);
+    };
+    load(k, data + (int64_t)min(kt0 + wave, kt1) * BYTES);
+    start_rows(a, x, r);
+    for (int kt = kt0 + wave; kt <= kt1; kt += 4) {
+        load(v, data + (int64_t)kt * BYTES + HALF);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r.s[kb][i] = 0.0f;
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                r.s[kb] = mfma<E>(k[kb * NM + m], r.q[0][m], r.s[kb]);
+                if constexpr (NP == 2) {
+                    r.s[kb] = mfma<E>(k[kb * NM + m], r.q[1][m], r.s[kb]);
+                    r.s[kb] = mfma<E>(k[PLANE + kb * NM + m], r.q[0][m], r.s[kb]);
+                }
+            }
+        load(k, data + (int64_t)min(kt + 4, kt1) * BYTES);
+        if (kt - words_at >= 64) {
+            words_at += 64;
+            words = a.info[tile0 + min(words_at + lane, kt1)];
+        }
+        const TileInfo info{__builtin_amdgcn_readlane(words, kt - words_at)};
+        weights(a, kt, info, r);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < ND; ++t) {
+                r.o[t] = mfma<E>(v[t * U + u], r.p[0][u], r.o[t]);
+                if constexpr (NP == 2) {
+                    r.o[t] = mfma<E>(v[t * U + u], r.p[1][u], r.o[t]);
+                    r.o[t] = mfma<E>(v[PLANE + t * U + u], r.p[0][u], r.o[t]);
+                }
+            }
+        if (info.odd()) strange_values(a, p, head, kt, r);
+    }
+
+    // the waves' parts, to one maximum
+    const float l = halves_sum(r.l);
+    lds_m[wave][lane] = r.m;
+    lds_l[wave][lane] = l;
+    __syncthreads();
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, lds_m[w][lane]);
+    // (a maximum of -inf: no key, or NaN, which the sum keeps)
+    auto by = [&](float of) { return of > -INFINITY ? __builtin_amdgcn_exp2f(of - m) : 1.0f; };
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum += lds_l[w][lane] * by(lds_m[w][lane]);
+    float f = l != 0.0f ? by(r.m) : 0.0f;
+    if constexpr (NP == 2) f = l != 0.0f ? ldexpf(f, r.ev_ref - kTopExp - kPExp) : 0.0f;
+    const float g = sum != 0.0f ? 1.0f / sum : 0.0f;
+    T *out = (T *)a.out + (p.start + r.token) * a.out_stride + (head * group + hq) * D + 4 * (lane >> 5);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4 * OWN; ++i) parts[wave][i][lane] = r.o[h * ND / 2 + i / 16][i % 16] * f;
+        __syncthreads();
+        if (row < rows)
+#pragma unroll
+            for (int b = 0; b < OWN / 4; ++b) {
+                const int at = wave * OWN + 4 * b, t = h * ND / 2 + at / 16;
+                T y[4] __attribute__((aligned(16)));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    y[i] = (T)((parts[0][at + i][lane] + parts[1][at + i][lane] + parts[2][at + i][lane] + parts[3][at + i][lane]) * g);
+                T *to = out + 32 * t + 8 * (at % 16 / 4);
+                if constexpr (sizeof(T) == 4)
+                    *(float4 *)to = *(const float4 *)y;
+                else
+                    *(uint2 *)to = *(const uint2 *)y;
+            }
+    }
+}
+
 template <typename T, int D> hipError_t prompt_launch(const PromptArgs &a, hipStream_t st) {
     k_prompt_pack<T, D><<<dim3((unsigned)a.n_tiles, (unsigned)a.n_kv_heads), 256, 0, st>>>(a);
-    k_prompt_attn<T, D><<<(unsigned)(a.n_slots * a.n_kv_heads), kPromptThreads, 0, st>>>(a);
+    const unsigned groups = (unsigned)(a.n_slots * a.n_kv_heads);
+    a.rows == kPromptRows ? k_prompt_attn<T, D><<<groups, kPromptThreads, 0, st>>>(a) : k_prompt_attn_few<T, D><<<groups, 256, 0, st>>>(a);
     return hipGetLastError();
 }
 

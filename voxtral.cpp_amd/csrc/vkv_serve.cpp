@@ -105,6 +105,14 @@ template <typename P> P *layer_at(P *base, const vkv_pages *p, int32_t layer, in
     return base + (int64_t)layer * p->n_pages * p->n_kv_heads * per_head;
 }
 
+// Up to so many work groups of kPromptRows rows, which leave CUs idle, prompts
+// of more than a tile of keys go by kPromptRowsFew rows and their keys over the
+// waves (f32, 32 heads over 8 of 128: 200 tokens 56 work groups, 21.0 -> 15.8 us;
+// 700 tokens 176, 45.3 -> 41.9; 1000 tokens 256, 61.3 against 63.2; bf16 200
+// tokens 13.4 -> 11.0, 700 tokens 25.8 against 27.9, 1500 tokens 376, 45.6
+// against 62.1; a single token 8.9 against 10.5).
+constexpr int64_t kPromptGroupsFew = 192;
+
 // Work groups of the paged attention beyond which longer chunks only save
 // partials: four per CU (16 rows of 8192 tokens 40.8 us, 46.3 with twice as
 // many; 131 rows of up to 500 21.4 us, 30.5).  A chunk's start and end, and its
@@ -296,8 +304,12 @@ vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const
     if (n_seq < 0 || n_tokens < 0 || window < 0) return bad("%s: %d prompts of %d tokens, window %d", what, n_seq, n_tokens, window);
     if (!std::isfinite(scale)) return bad("%s: scale", what);
     PromptArgs a{};
-    a.n_tiles = prompt_tiles(n_seq, n_tokens, prompt_keys(prompt_planes(dtype), head_dim));
-    a.n_slots = (int64_t)n_tokens * (n_q_heads / n_kv_heads) / kPromptRows + n_seq;
+    const int keys = prompt_keys(prompt_planes(dtype), head_dim);
+    a.n_tiles = prompt_tiles(n_seq, n_tokens, keys);
+    const int64_t rows = (int64_t)n_tokens * (n_q_heads / n_kv_heads);
+    const bool few = (rows / kPromptRows + n_seq) * n_kv_heads <= kPromptGroupsFew && n_tokens > keys;
+    a.rows = few ? kPromptRowsFew : kPromptRows;
+    a.n_slots = rows / a.rows + n_seq;
     if (a.n_tiles >= 1 << 24 || a.n_slots * n_kv_heads >= 1 << 23) return bad("%s: %d prompts of %d tokens", what, n_seq, n_tokens);
     if (n_seq == 0 || n_tokens == 0) return host_ok();
     if (vkv_status s = check_ints(what, cu_seqlens)) return s;

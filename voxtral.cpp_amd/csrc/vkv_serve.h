@@ -58,7 +58,8 @@ struct PagedAttnArgs {
 hipError_t launch_paged_attn(int dtype, int code, int head_dim, const PagedAttnArgs &a, hipStream_t st);
 
 // Causal attention of packed prompts (vkv_prompt.hip).
-constexpr int kPromptRows = 128;    // (token, query head of a kv head) rows per work group
+// (token, query head of a kv head) rows per work group, and where they are few
+constexpr int kPromptRows = 128, kPromptRowsFew = 32;
 // Keys per tile: of K and V, `planes` 16-bit planes each, two tiles take 64 KiB
 constexpr int prompt_keys(int planes, int head_dim) { return planes * head_dim <= 128 ? 64 : 32; }
 
@@ -69,6 +70,7 @@ struct PromptArgs {
     const int32_t *cu;
     int32_t n_seq, n_tokens, n_q_heads, n_kv_heads, window;
     int64_t n_tiles;       // key tiles of a kv head
+    int32_t rows;          // of a query tile
     int64_t n_slots;       // query tiles of a kv head
     float scale;
     int32_t *info;         // [kv head][tile]: exponents of K and V, whether V holds what is not finite
