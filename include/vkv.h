@@ -827,8 +827,9 @@ typedef struct vkv_pages {
  * [cu_new[n_req], max_tokens).  len_out (which may be len_old or len_new)
  * receives the requests' lengths.
  * *status = 0; or 1 where the free pages do not suffice, 2 where a length is
- * negative or beyond the table, the new tokens are more than max_tokens, or
- * the stack or a returned entry is no page's: then nothing moves, len_out =
+ * negative or beyond the table, the new tokens are more than max_tokens, a
+ * returned entry is no page's id, or the stack's size is out of range (the ids
+ * on it are taken as they are): then nothing moves, len_out =
  * len_old, every offset is 0 and every slot -1, so that the step's other calls
  * do nothing. */
 vkv_status vkv_page_map(const int32_t *len_old, const int32_t *len_new, int32_t n_req,
@@ -863,7 +864,8 @@ vkv_status vkv_pages_append(const vkv_pages *pages, int32_t layer, const int32_t
  * max_len <= table_stride * page_size (with stride 0: the one table's pages
  * are taken to reach max_len).  q, out: [n_rows][n_q_heads][head_dim]; the
  * products take q and the softmax weights in 22 bits, sums are 32-bit.
- * The workspace is 16-byte aligned; its contents do not matter. */
+ * The workspace is 16-byte aligned; its contents do not matter; one for n_rows
+ * and max_len does for fewer of either and for any window. */
 size_t vkv_paged_attn_workspace(const vkv_pages *pages, int32_t n_rows, int32_t n_q_heads,
                                 int32_t max_len);
 vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *table,
@@ -886,7 +888,8 @@ vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *
  * 32 or 64 neighbouring keys; steps of 2^-37 of that largest below.  F16 and
  * BF16 rows are multiplied as they are, with the softmax weights rounded to
  * that type.  Sums are 32-bit.
- * The workspace is 256-byte aligned; its contents do not matter. */
+ * The workspace is 256-byte aligned; its contents do not matter; one for n_seq
+ * and n_tokens does for fewer of either. */
 size_t vkv_prompt_attn_workspace(int32_t dtype, int32_t n_seq, int32_t n_tokens,
                                  int32_t n_kv_heads, int32_t head_dim);
 vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const void *k,
@@ -905,7 +908,8 @@ vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const
  * +inf in a row makes its log probabilities and entropy NaN (NaN counts as the
  * largest).  The log probability of token -1 (a padding row) is 0, of any
  * other id outside the vocabulary NaN.
- * The workspace is 16-byte aligned; its contents do not matter. */
+ * The workspace is 16-byte aligned; its contents do not matter; one for n_rows
+ * and n_top does for fewer of either. */
 #define VKV_LOGPROBS_MAX_TOP 32
 size_t vkv_logprobs_workspace(int32_t n_rows, int64_t n_vocab, int32_t n_top);
 vkv_status vkv_logprobs(int32_t dtype, const void *logits, int64_t row_stride, int32_t n_rows,

@@ -134,6 +134,40 @@ def test_logprobs_workspace():
     assert vkv.logprobs_workspace(-1, 1000, 3) == 0
 
 
+def large_enough(call):
+    """the size is accepted: the missing pointer, looked at next, is what the call refuses"""
+    refused(call, vkv.INVALID_ARGUMENT, "workspace null")
+
+
+def test_a_workspace_does_for_smaller_batches():
+    for heads, kv in ((32, 8), (32, 32), (16, 1), (9, 3)):
+        p = pages(n_pages=100000, n_kv_heads=kv)
+        for most, longest in ((19, 8192), (64, 8192), (200, 1000), (1100, 300), (3, 100000)):
+            need = vkv.paged_attn_workspace(p, most, heads, longest)
+            for rows in {1, 2, 3, 5, 8, 16, 17, 18, 63, most // 2, most - 1, most}:
+                for max_len in {257, 300, 1000, longest // 3, longest - 1, longest}:
+                    for window in (0, 1, 255, 256, 1000, longest - 1):
+                        # (a plan of one chunk needs none and refuses nothing here)
+                        span = min(max_len, window + 31) if window else max_len
+                        if not 0 < rows <= most or max_len > longest or span <= 1024:
+                            continue
+                        large_enough(lambda: vkv.paged_attn(p, 0, A, 8192, A, rows, max_len, vkv.F32, A, A, heads, 0.1,
+                                                            window, 0, need))
+    for most, vocab, top in ((17, 131072, 5), (251, 131072, 20), (64, 32003, 32), (2000, 5001, 32), (65535, 300, 3), (3, 1 << 30, 1)):
+        need = vkv.logprobs_workspace(most, vocab, top)
+        for rows in {1, 2, 3, 7, 8, 16, 31, 64, 200, most // 2, most - 1, most}:
+            for fewer in {0, 1, top // 2, top}:
+                for dtype in (vkv.F32, vkv.BF16):
+                    for stride in (0, vocab + 1, vocab + 8):
+                        if 0 < rows <= most:
+                            large_enough(lambda: vkv.logprobs(dtype, A, rows, vocab, A, A, A, fewer, A, A, 0, need, row_stride=stride))
+    for dtype in (vkv.F32, vkv.F16):
+        need = vkv.prompt_attn_workspace(dtype, 9, 5000, 8, 128)
+        for seqs in (1, 4, 9):
+            for tokens in (1, 63, 1000, 5000):
+                large_enough(lambda: vkv.prompt_attn(dtype, A, A, A, A, seqs, tokens, 32, 8, 128, 0.1, 0, A, 0, need))
+
+
 def test_empty_calls_do_nothing():
     vkv.pages_append(pages(), 0, 0, 0, vkv.F32, 0, 0)
     vkv.paged_attn(pages(), **{**ATTN, "n_rows": 0})

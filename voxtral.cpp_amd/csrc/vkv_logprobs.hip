@@ -485,6 +485,19 @@ LogprobsPlan logprobs_plan(int n_rows, int64_t n_vocab, int elem_bytes, int n_to
     return p;
 }
 
+int64_t logprobs_chunks_most(int64_t n_rows, int64_t n_vocab) {
+    int64_t most = 0;
+    for (int per : {4, 8}) {
+        const int64_t blocks = (n_vocab + 2 * (per - 1)) / per;
+        const int64_t small = (blocks + kBlocksFew * kThreads - 1) / (kBlocksFew * kThreads);
+        const int64_t large = (blocks + 32 / per * kThreads - 1) / (32 / per * kThreads);
+        // a chunk of `turns` pieces: turns is 1, its most, or at least what leaves kManyGroups chunks
+        const int64_t many = std::max(n_rows * ((large + kTurnsMost - 1) / kTurnsMost), std::min(n_rows * large, kManyGroups + n_rows));
+        most = std::max(most, std::max(std::min(n_rows * small, kFewGroups), many));
+    }
+    return most;
+}
+
 hipError_t launch_logprobs(int dtype, const LogprobsArgs &a, int blocks, hipStream_t st) {
     if (dtype == VKV_DTYPE_F16) return run<_Float16>(a, blocks, st);
     if (dtype == VKV_DTYPE_BF16) return run<__bf16>(a, blocks, st);

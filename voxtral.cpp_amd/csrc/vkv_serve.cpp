@@ -136,15 +136,16 @@ void attn_plan(int64_t units, int32_t max_len, int32_t window, int32_t *chunk, i
     *n_chunks = (int32_t)((span + c - 1) / c);
 }
 
-// no fewer chunks than any window's plan has
-int64_t attn_chunks_most(int64_t units, int32_t max_len) {
+// No fewer (row, chunk) pairs than any plan of so many rows and tokens, or of
+// fewer, has, with any window: a chunk is at its least, its most, or at
+// least what leaves kAttnGroups units, `per_row` to a row.
+int64_t attn_parts_most(int64_t n_rows, int64_t per_row, int32_t max_len) {
     const int64_t span = (int64_t)max_len + 31;
-    const int64_t few = (span + kPagedChunkMax - 1) / kPagedChunkMax;
-    const int64_t many = std::min<int64_t>((span + kAttnChunkMin - 1) / kAttnChunkMin, kAttnGroups / std::max<int64_t>(units, 1) + 1);
-    return std::max(few, many);
+    const int64_t few = (span + kPagedChunkMax - 1) / kPagedChunkMax, many = (span + kAttnChunkMin - 1) / kAttnChunkMin;
+    return std::max(n_rows * few, std::min(n_rows * many, kAttnGroups / per_row + n_rows));
 }
 
-int64_t attn_bytes(int64_t rows_heads, int64_t chunks, int32_t head_dim) { return rows_heads * chunks * (head_dim + 2) * 4; }
+int64_t attn_bytes(int64_t parts, int32_t n_q_heads, int32_t head_dim) { return parts * n_q_heads * (head_dim + 2) * 4; }
 
 int prompt_planes(int32_t dtype) { return dtype == VKV_DTYPE_F32 ? 2 : 1; }
 int64_t prompt_tiles(int32_t n_seq, int32_t n_tokens, int keys) { return (int64_t)n_tokens / keys + n_seq; }
@@ -153,8 +154,8 @@ int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 int64_t prompt_info_bytes(int64_t tiles, int32_t n_kv_heads) { return round256(tiles * n_kv_heads * 4); }
 
-// (maximum, sum, weighted sum) of each wave
-int64_t logprobs_stats_bytes(int64_t n_rows, int64_t chunks) { return n_rows * chunks * 4 * 16; }
+// a chunk's (maximum, sum, weighted sum, count) of each of 4 waves
+int64_t logprobs_stats_bytes(int64_t chunks) { return chunks * 4 * 16; }
 
 }  // namespace
 
@@ -220,8 +221,8 @@ size_t vkv_paged_attn_workspace(const vkv_pages *pages, int32_t n_rows, int32_t 
     if (check_pool("paged attention workspace", pages) || n_rows < 0 || max_len < 0 ||
         check_heads("paged attention workspace", n_q_heads, pages->n_kv_heads))
         return 0;
-    const int64_t most = attn_chunks_most(attn_units(n_rows, n_q_heads, pages->n_kv_heads), max_len);
-    return (size_t)attn_bytes((int64_t)n_rows * n_q_heads, most, pages->head_dim);
+    const int64_t most = attn_parts_most(n_rows, attn_units(1, n_q_heads, pages->n_kv_heads), max_len);
+    return (size_t)attn_bytes(most, n_q_heads, pages->head_dim);
 }
 
 vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *table, int32_t table_stride,
@@ -252,7 +253,7 @@ vkv_status vkv_paged_attn(const vkv_pages *pages, int32_t layer, const int32_t *
     if ((units + 8 * (units / n_rows)) * a.n_chunks >= 1 << 24) return bad("%s: %d rows of up to %d tokens", what, n_rows, max_len);
     const int64_t parts = (int64_t)n_rows * n_q_heads * a.n_chunks;
     if (a.n_chunks > 1) {
-        const int64_t need = attn_bytes((int64_t)n_rows * n_q_heads, a.n_chunks, pages->head_dim);
+        const int64_t need = attn_bytes((int64_t)n_rows * a.n_chunks, n_q_heads, pages->head_dim);
         if ((int64_t)workspace_bytes < need) return small_ws(what, workspace_bytes, (size_t)need);
         if (!workspace || !aligned(workspace, 16)) return bad("%s: workspace null or not 16-byte aligned", what);
     }
@@ -346,11 +347,8 @@ vkv_status vkv_prompt_attn(int32_t dtype, const void *q, int64_t q_stride, const
 
 size_t vkv_logprobs_workspace(int32_t n_rows, int64_t n_vocab, int32_t n_top) {
     if (n_rows < 0 || n_vocab < 1 || n_vocab > 1 << 30 || n_top < 0 || n_top > kLogprobsMaxTop) return 0;
-    int64_t most = 0;
-    for (int eb : {2, 4})
-        for (bool aligned_rows : {false, true})
-            most = std::max<int64_t>(most, logprobs_plan(n_rows, n_vocab, eb, n_top, aligned_rows).chunks);
-    return (size_t)(logprobs_stats_bytes(n_rows, most) + n_rows * most * n_top * 8);
+    const int64_t most = logprobs_chunks_most(n_rows, n_vocab);
+    return (size_t)(logprobs_stats_bytes(most) + most * n_top * 8);
 }
 
 vkv_status vkv_logprobs(int32_t dtype, const void *logits, int64_t row_stride, int32_t n_rows, int64_t n_vocab,
@@ -373,8 +371,8 @@ vkv_status vkv_logprobs(int32_t dtype, const void *logits, int64_t row_stride, i
     if (!aligned(tokens, 4) || !aligned(logprob, 4) || !aligned(entropy, 4))
         return bad("%s: int32 and f32 arrays must be 4-byte aligned", what);
     const LogprobsPlan plan = logprobs_plan(n_rows, n_vocab, eb, n_top, n_rows == 1 || row_stride * eb % 16 == 0);
-    const int64_t chunks = plan.chunks;
-    const int64_t stats = logprobs_stats_bytes(n_rows, chunks), need = stats + n_rows * chunks * n_top * 8;
+    const int64_t chunks = (int64_t)n_rows * plan.chunks;
+    const int64_t stats = logprobs_stats_bytes(chunks), need = stats + chunks * n_top * 8;
     if ((int64_t)workspace_bytes < need) return small_ws(what, workspace_bytes, (size_t)need);
     if (!workspace || !aligned(workspace, 16)) return bad("%s: workspace null or not 16-byte aligned", what);
     LogprobsArgs a{logits, row_stride, n_rows, (int32_t)n_vocab, n_top, plan.chunks, plan.turns, tokens, logprob, entropy,

@@ -100,6 +100,8 @@ struct LogprobsPlan {
     int32_t blocks, turns, chunks;
 };
 LogprobsPlan logprobs_plan(int n_rows, int64_t n_vocab, int elem_bytes, int n_top, bool rows_aligned);
+// no fewer chunks than any plan of so many rows, or of fewer, has
+int64_t logprobs_chunks_most(int64_t n_rows, int64_t n_vocab);
 hipError_t launch_logprobs(int dtype, const LogprobsArgs &a, int blocks, hipStream_t st);
 
 }  // namespace vkv
