@@ -444,23 +444,26 @@ template <int FMT> __device__ __forceinline__ int scale_exponent(float amax) {
 
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= FLT_MAX; }
 
-// four values in units of the scale to four codes (nearest, ties to even)
-template <int FMT> __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
+// Four values in units of the scale to four codes (nearest, ties to even).
+// FINE: all are finite.  An int8 code is the low byte of x + 1.5 * 2^23, whose
+// step is 1.
+template <int FMT, bool FINE> __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
     if constexpr (FMT == VKV_DTYPE_E4M3) {
-        const float nan = __builtin_nanf("");
-        a = is_finite(a) ? a : nan;
-        b = is_finite(b) ? b : nan;
-        c = is_finite(c) ? c : nan;
-        d = is_finite(d) ? d : nan;
+        if constexpr (!FINE) {
+            const float nan = __builtin_nanf("");
+            a = is_finite(a) ? a : nan;
+            b = is_finite(b) ? b : nan;
+            c = is_finite(c) ? c : nan;
+            d = is_finite(d) ? d : nan;
+        }
         unsigned r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
         return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
     } else {
         auto one = [](float x) -> unsigned {
-            x = x == x ? x : 0.0f;
-            x = fminf(fmaxf(rintf(x), -127.0f), 127.0f);
-            return (unsigned)(int)x & 255u;
+            if (!FINE) x = x == x ? x : 0.0f;
+            return __float_as_uint(__builtin_amdgcn_fmed3f(x, -127.0f, 127.0f) + 12582912.0f);
         };
-        return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+        return __builtin_amdgcn_perm(one(b), one(a), 0x0c0c0400u) | __builtin_amdgcn_perm(one(d), one(c), 0x04000c0cu);
     }
 }
 
@@ -482,7 +485,7 @@ template <int FMT> __device__ __forceinline__ void unpack4(unsigned w, float v[4
 template <int FMT> __device__ __forceinline__ unsigned rescale4(unsigned w, float down) {
     float v[4];
     unpack4<FMT>(w, v);
-    return pack4<FMT>(v[0] * down, v[1] * down, v[2] * down, v[3] * down);
+    return pack4<FMT, false>(v[0] * down, v[1] * down, v[2] * down, v[3] * down);
 }
 
 // ---------------------------------------------------------------------------
@@ -519,9 +522,11 @@ template <typename T, int N> struct Raw {
 // dim are a word of V's stored order.
 //
 // Few tokens are bound by latency: slots, rows, and the page's waves' meeting
-// (32 of 8 x 128 f32 values 4.8 us, 2.5 of them an empty launch's).  4099
-// tokens of prompts, bf16 to int8 pages of 64: 14 us for 25 MB, 1.8 TB/s: the
-// search for the runs ends after 5.0 us, the rows are there after 9.9.
+// (32 of 8 x 128 f32 values 4.6 us, 2.5 of them an empty launch's).  4099
+// tokens of prompts, bf16 to int8 pages of 64: 12.6 us for 25 MB, 2.0 TB/s: the
+// search for the runs ends after 5 us, the rows are there after 9.  Finite rows
+// are told by one maximum of their bits and rounded without a test for each
+// value (14.0 us with one).
 template <typename T, int FMT, int D>
 __global__ __launch_bounds__(1024) void k_pages_append(AppendPagesArgs a) {
     constexpr int N = D / 16;
@@ -581,15 +586,22 @@ __global__ __launch_bounds__(1024) void k_pages_append(AppendPagesArgs a) {
                     is_v ? ((const unsigned *)codes)[(((c * N + i) % 16) * 4 + g) * N + (c * N + i) / 16]
                          : ((const unsigned *)(codes + (4 * g + i / (N / 4)) * D + c * N))[i % (N / 4)];
         }
-        float amax = 0.0f;
+        unsigned most = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (rows[j] >= 0)
 #pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const float y = fabsf(x[j][n]);
-                    amax = fmaxf(amax, y <= FLT_MAX ? y : 0.0f);
-                }
+                for (int n = 0; n < N; ++n) most = max(most, __float_as_uint(x[j][n]) & 0x7fffffffu);
+        const bool fine = !__any(most >= 0x7f800000u);
+        float amax = __uint_as_float(most);
+        if (!fine) {
+            amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (rows[j] >= 0)
+#pragma unroll
+                    for (int n = 0; n < N; ++n) amax = fmaxf(amax, is_finite(x[j][n]) ? fabsf(x[j][n]) : 0.0f);
+        }
         amax = wave_max(amax);
         if (blocks > 1) {
             __syncthreads();
@@ -607,39 +619,43 @@ __global__ __launch_bounds__(1024) void k_pages_append(AppendPagesArgs a) {
         const bool grown = down != 1.0f;
         const float inv = exp2_int(-e);
         if (b == 0 && lane == 0) *scale = exp2_int(e);
-        if (!is_v) {
+        auto store = [&](auto is_fine) {
+            constexpr bool FINE = decltype(is_fine)::value;
+            if (!is_v) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (rows[j] >= 0 || grown) {
-                    unsigned w[N / 4];
+                for (int j = 0; j < 4; ++j)
+                    if (rows[j] >= 0 || grown) {
+                        unsigned w[N / 4];
 #pragma unroll
-                    for (int n = 0; n < N / 4; ++n)
-                        w[n] = rows[j] >= 0 ? pack4<FMT>(x[j][4 * n] * inv, x[j][4 * n + 1] * inv, x[j][4 * n + 2] * inv,
-                                                         x[j][4 * n + 3] * inv)
-                                            : rescale4<FMT>(old[j][n], down);
-                    unsigned *dst = (unsigned *)(codes + (4 * g + j) * D + c * N);
-                    if constexpr (N == 8)
-                        *(uint2 *)dst = uint2{w[0], w[1]};
-                    else
-                        *dst = w[0];
-                }
-        } else {
-            unsigned mask = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mask |= rows[j] >= 0 ? 255u << 8 * j : 0u;
-            if (mask != 0 || grown)
-#pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    unsigned y = pack4<FMT>(rows[0] >= 0 ? x[0][n] * inv : 0.0f, rows[1] >= 0 ? x[1][n] * inv : 0.0f,
-                                            rows[2] >= 0 ? x[2][n] * inv : 0.0f, rows[3] >= 0 ? x[3][n] * inv : 0.0f);
-                    if (!whole) {
-                        unsigned w = old[n / (N / 4)][n % (N / 4)];
-                        if (grown) w = rescale4<FMT>(w, down);
-                        y = (w & ~mask) | (y & mask);
+                        for (int n = 0; n < N / 4; ++n)
+                            w[n] = rows[j] >= 0 ? pack4<FMT, FINE>(x[j][4 * n] * inv, x[j][4 * n + 1] * inv, x[j][4 * n + 2] * inv,
+                                                             x[j][4 * n + 3] * inv)
+                                                : rescale4<FMT>(old[j][n], down);
+                        unsigned *dst = (unsigned *)(codes + (4 * g + j) * D + c * N);
+                        if constexpr (N == 8)
+                            *(uint2 *)dst = uint2{w[0], w[1]};
+                        else
+                            *dst = w[0];
                     }
-                    ((unsigned *)codes)[(((c * N + n) % 16) * 4 + g) * N + (c * N + n) / 16] = y;
-                }
-        }
+            } else {
+                unsigned mask = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mask |= rows[j] >= 0 ? 255u << 8 * j : 0u;
+                if (mask != 0 || grown)
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        unsigned y = pack4<FMT, FINE>(rows[0] >= 0 ? x[0][n] * inv : 0.0f, rows[1] >= 0 ? x[1][n] * inv : 0.0f,
+                                                rows[2] >= 0 ? x[2][n] * inv : 0.0f, rows[3] >= 0 ? x[3][n] * inv : 0.0f);
+                        if (!whole) {
+                            unsigned w = old[n / (N / 4)][n % (N / 4)];
+                            if (grown) w = rescale4<FMT>(w, down);
+                            y = (w & ~mask) | (y & mask);
+                        }
+                        ((unsigned *)codes)[(((c * N + n) % 16) * 4 + g) * N + (c * N + n) / 16] = y;
+                    }
+            }
+        };
+        if (fine) store(std::true_type{}); else store(std::false_type{});
     }
 }
 
