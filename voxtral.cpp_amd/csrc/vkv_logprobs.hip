@@ -22,7 +22,9 @@ typedef unsigned long long u64;
 constexpr int kThreads = 256;
 // Pieces: 2 blocks per thread where that makes few work groups (a row or a
 // few: the time is latency) whose lists k_logprobs_join takes in one turn (a
-// row in f32, n_top 20: 12.1 us, 16.0 with 64 work groups), else 32 elements per thread, as many pieces per
+// row in f32, n_top 5: 9.8 us, 11.0 with the larger pieces; n_top 20, two turns:
+// 16.0 us, 11.7 with the larger pieces; 32 rows, n_top 5, beyond kFewGroups:
+// 14.9 us, 12.1 with them), else 32 elements per thread, as many pieces per
 // work group as leave kManyGroups of them, which run at the same time (rows of
 // 131072 logits in bf16, n_top 20, both launches: 251 rows 23.4 us, 29.1 with
 // twice the work groups, 29.1 with 3/4; 512 rows 32.4 us, 35.7 where a work
@@ -346,6 +348,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
 // keys of the chunks' lists per thread and turn: with the largest so far, a
 // wave's fit its piece
 constexpr int kJoinPer = 3;
+// up to so many keys go to the list all together, without a limit (160 keys of
+// a bf16 row 12.1 us, 10.2 with one; 80 of 251 rows 25.4 us, 25.8 with one)
+constexpr int kJoinAll = 128;
 
 // A wave's, or several waves', elements: the maximum m, how many there are of
 // it, and of the others the sums of exp(x - m) and (x - m) exp(x - m).  The
@@ -427,7 +432,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(LogprobsArgs a) {
         for (int i = 0; i < kJoinPer; ++i) best = k[i] > best ? k[i] : best;
         u64 least = 1;
         __syncthreads();
-        if (n_keys > kThreads) {        // (else the list takes them all)
+        if (n_keys > kJoinAll) {
             search.x[tid] = (unsigned)(best >> 32);
             __syncthreads();
             search_nth(search, a.n_top);
