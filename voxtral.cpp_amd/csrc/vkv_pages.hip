@@ -419,9 +419,8 @@ __global__ __launch_bounds__(256) void k_map_tokens(MapArgs a) {
 // Codes and scales
 // ---------------------------------------------------------------------------
 
+// FMT below: VKV_DTYPE_E4M3 or VKV_DTYPE_I8
 constexpr int kScaleMin = -100, kScaleMax = 120;   // exponents of a scale
-
-template <int FMT> struct Code;   // FMT: VKV_DTYPE_E4M3 or VKV_DTYPE_I8
 
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float scale) {
