@@ -374,6 +374,26 @@ def test_logprobs_of_large_logits(vocab, rows):
     check_logprobs(x, rng.integers(0, vocab, rows), 3, vkv.F32)
 
 
+@pytest.mark.parametrize("dtype", [vkv.F32, vkv.F16])
+@pytest.mark.parametrize("vocab,rows", [(999, 12), (30001, 12), (30001, 250)])
+def test_logprobs_of_rows_of_equal_values(vocab, rows, dtype):
+    """masks of the type's lowest value with a few logits left, more or fewer than are asked for; rows of one value; two
+    values; equal values in many places and pieces"""
+    rng = np.random.default_rng(16)
+    low = float(torch.finfo(TORCH[dtype]).min)
+    x = np.full((rows, vocab), low)
+    for r in range(rows):
+        kind = r % 6
+        some = rng.permutation(vocab)[:[3, 32, 200, 0, 40, 17][kind]]
+        if kind < 3:
+            x[r, some] = rng.standard_normal(len(some))
+        else:
+            x[r] = 0.0
+            x[r, some] = 1.0 if kind == 4 else rng.integers(0, 3, len(some))
+    check_logprobs(x, rng.integers(0, vocab, rows), 32, dtype)
+    check_logprobs(x, rng.integers(0, vocab, rows), 5, dtype)
+
+
 def test_logprobs_masked_rows():
     """-inf has no probability; a row of it alone has no distribution; NaN and +inf make a row NaN"""
     rng = np.random.default_rng(4)

@@ -83,12 +83,17 @@ struct List {
     __attribute__((aligned(16))) int count[kWaves];
 };
 
+// how many of the lanes below this one are in the set
+__device__ __forceinline__ int lanes_below(u64 set) {
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(set >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)set, 0));
+}
+
 // The wave's elements for which `take` holds go to its piece, as far as it has
 // room; `kept` counts them all.
 template <typename Take, typename Key> __device__ __forceinline__ void put(List &list, int &kept, Take take, Key key) {
     const u64 on = __ballot(take);
     if (on == 0) return;
-    const int at = kept + __builtin_amdgcn_mbcnt_hi((unsigned)(on >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)on, 0));
+    const int at = kept + lanes_below(on);
     if (take && at < kPiece) list.key[threadIdx.x >> 6][at] = key();
     kept += __popcll(on);
 }
@@ -126,8 +131,8 @@ __device__ __forceinline__ void rank(const List &list, int n, u64 *out) {
 }
 
 // The n largest of the row's elements [from, to) one after the other, each the
-// largest below the last: for chunks with so many equal values that a list
-// does not hold them, or NaN.
+// largest below the last: for chunks with more elements above the limit than a
+// list holds (they rise, and the limit is the first piece's), NaN or +inf.
 template <typename T> __device__ __noinline__ void pick(const T *x, int64_t from, int64_t to, int n, u64 *wave_best, u64 *out) {
     u64 last = ~0ull;
     for (int r = 0; r < n; ++r) {
@@ -160,7 +165,9 @@ template <typename T> __device__ __noinline__ void pick(const T *x, int64_t from
 // piece, by one wave while the others sum, it is the limit for all.  The blocks
 // with elements that are not below it, a few more than n per piece as a rule,
 // are set aside whole, one test for a block; at the end their elements go to a
-// list that is ranked by counting.
+// list that is ranked by counting.  Equal values rank by rising index, so of
+// those that equal the limit (masked logits of the type's lowest value, a row
+// of zeros) each wave keeps its first n.
 //
 // Bound by the vector units beside the loads, about 8 instructions and one
 // exponential for an element: 251 rows of 131072 logits in bf16 with 20
@@ -194,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
     uint4 next[BLOCKS];
     load(chunk0, next);
     float m = -INFINITY, s = 0.0f, t = 0.0f, n = 0.0f, limit = -INFINITY, largest = -INFINITY;
-    int kept = 0, set_aside = 0;
+    int kept = 0, set_aside = 0, even_blocks = 0;
     for (int piece = chunk0; piece < end; piece += PIECE) {
         float v[PER];
 #pragma unroll
@@ -286,10 +293,13 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
         if (limit > -INFINITY) {
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
-                const bool take = of_block[b] >= limit;
+                if (!__any(of_block[b] >= limit)) continue;
+                // of the blocks that only reach the limit the wave's first n are enough
+                const u64 even = __ballot(of_block[b] == limit);
+                const bool take = of_block[b] > limit || (of_block[b] == limit && even_blocks + lanes_below(even) < a.n_top);
+                even_blocks += __popcll(even);
                 const u64 on = __ballot(take);
-                if (on == 0) continue;
-                const int at = set_aside + __builtin_amdgcn_mbcnt_hi((unsigned)(on >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)on, 0));
+                const int at = set_aside + lanes_below(on);
                 if (take && at < kHot) {
                     T y[EB] __attribute__((aligned(16)));
 #pragma unroll
@@ -321,14 +331,25 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
         __syncthreads();
         limit = fmaxf(limit, value_of(search.found));
     }
+    int even_before = 0;
     for (int i = tid & 63; i - (tid & 63) < min(set_aside, kHot); i += 64) {
         const bool in = i < min(set_aside, kHot);
         const uint4 y = hot.block[tid >> 6][min(i, kHot - 1)];
         const int first = hot.first[tid >> 6][min(i, kHot - 1)];
+        // (and of the elements, in their order)
+        float z[EB];
+        int even = even_before;
 #pragma unroll
         for (int q = 0; q < EB; ++q) {
-            const float z = (float)((const T *)&y)[q];
-            put(list, kept, in && z >= limit, [&] { return key_of(z, (unsigned)(first + q)); });
+            z[q] = in ? (float)((const T *)&y)[q] : -INFINITY;
+            const u64 on = __ballot(z[q] == limit);
+            even += lanes_below(on);
+            even_before += __popcll(on);
+        }
+#pragma unroll
+        for (int q = 0; q < EB; ++q) {
+            put(list, kept, z[q] > limit || (z[q] == limit && even < a.n_top), [&] { return key_of(z[q], (unsigned)(first + q)); });
+            even += z[q] == limit;
         }
     }
     if ((tid & 63) == 0) {
