@@ -167,11 +167,11 @@ template <typename T> __device__ __noinline__ void pick(const T *x, int64_t from
 // are set aside whole, one test for a block; at the end their elements go to a
 // list that is ranked by counting.  Equal values rank by rising index, so of
 // those that equal the limit (masked logits of the type's lowest value, a row
-// of zeros) each wave keeps its first n.
+// of zeros) each wave keeps its first n (251 rows of zeros as below 34 us).
 //
 // Bound by the vector units beside the loads, about 8 instructions and one
 // exponential for an element: 251 rows of 131072 logits in bf16 with 20
-// alternatives 21 us, 3.1 TB/s (12 us without alternatives), 2 of them for the
+// alternatives 21.7 us, 3.0 TB/s (12 us without alternatives), 2 of them for the
 // maximum's terms kept apart.  One f32 row 5.3 us: a launch, a load, a search
 // and a ranking.
 template <typename T, int BLOCKS>
@@ -293,12 +293,16 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(LogprobsArgs a) {
         if (limit > -INFINITY) {
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
-                if (!__any(of_block[b] >= limit)) continue;
-                // of the blocks that only reach the limit the wave's first n are enough
-                const u64 even = __ballot(of_block[b] == limit);
-                const bool take = of_block[b] > limit || (of_block[b] == limit && even_blocks + lanes_below(even) < a.n_top);
-                even_blocks += __popcll(even);
-                const u64 on = __ballot(take);
+                bool take = of_block[b] >= limit;
+                u64 on = __ballot(take);
+                if (on == 0) continue;
+                if (set_aside + __popcll(on) > kHot / 2) {
+                    // many: of the blocks that only reach the limit the wave's next n are enough
+                    const u64 even = __ballot(of_block[b] == limit);
+                    take = take && (of_block[b] > limit || even_blocks + lanes_below(even) < a.n_top);
+                    even_blocks += __popcll(even);
+                    on = __ballot(take);
+                }
                 const int at = set_aside + lanes_below(on);
                 if (take && at < kHot) {
                     T y[EB] __attribute__((aligned(16)));
